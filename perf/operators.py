@@ -451,7 +451,7 @@ def _compact(s):
     if own:
         from freeml_b200 import kv4
         kv4.free(counts, table, lens, s["ended"], status)
-        kv4.compact(pool, counts, table, status)
+        kv4.compact(pool, counts, table)
         return meta, pool
     ended = s["ended"].long()
     rows = table[ended]
