@@ -137,6 +137,30 @@ def attention_prefill(out, q, kcache, vcache, prompt_len, scale, mode=None):
          _s())
 
 
+def attention_packed(out, q, k, v, starts, scale, k_starts=None, mode=None):
+    """Causal attention over packed prompts with grouped heads
+    (fml_attention_packed).  q/out: [rows, heads, hd], k/v: [rows, kv_heads,
+    hd], float32, float16 or bfloat16, heads dense (row strides free: views of
+    one QKV row will do); starts: int32 [batch + 1], the sequences' first rows;
+    k_starts: the same for k and v where their rows lead the queries (a prompt
+    run in chunks).  mode: FML_MATH_* of float32 (default: the library's)."""
+    from . import kv4
+    heads, kv_heads, hd = q.shape[1], k.shape[1], q.shape[2]
+    po, ldo = kv4._rows(out, heads, hd, "out")
+    pq, ldq = kv4._rows(q, heads, hd, "q")
+    pk, ldk = kv4._rows(k, kv_heads, hd, "k")
+    pv, ldv = kv4._rows(v, kv_heads, hd, "v")
+    _check(q.dtype in kv4.TYPES and out.dtype == k.dtype == v.dtype == q.dtype, "attention_packed types")
+    _check(out.shape[0] == q.shape[0] and k.shape[0] == v.shape[0] and
+           (k_starts is None or k_starts.shape == starts.shape), "attention_packed shapes")
+    if mode is None:
+        from ._lib import load
+        mode = int(load().fml_get_math_mode())
+    call("fml_attention_packed", po, pq, pk, pv, kv4.TYPES[q.dtype], kv4._ints(starts, "starts"),
+         kv4._ints(k_starts, "k_starts"), starts.shape[0] - 1, q.shape[0], k.shape[0], heads, kv_heads, hd, ldo, ldq, ldk,
+         ldv, float(scale), int(mode), _s())
+
+
 def attention_decode(out, q, kcache, vcache, lens, scale, workspace=None):
     """Causal attention of the newest row per sequence over a KV cache
     (fml_attention_decode).  q/out: [B, H*hd]; kcache/vcache: [B, H, C, hd];

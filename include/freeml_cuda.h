@@ -286,6 +286,125 @@ FML_API int fml_attention_prefill(float* out, const float* q, const float* kcach
                                   uint32_t batch, uint32_t heads, uint32_t head_dim, uint32_t context,
                                   uint32_t prompt_len, float scale, int mode, fml_stream_t stream);
 
+/* ---- Packed prompts and a 4-bit paged key/value cache -------------------
+ * No counterpart in the reference, which runs one window of one sequence:
+ * prompts of different lengths in one call with grouped heads, and a cache
+ * whose rows take 5 bits a value, held in pages that sequences share.  Tensor
+ * arguments are of one type, and sums, softmax statistics and the arithmetic
+ * between are fp32 for all three. */
+enum fml_type { FML_TYPE_FP32 = 0, FML_TYPE_FP16 = 1, FML_TYPE_BF16 = 2 };
+
+/* Causal attention over packed prompts with grouped heads:
+ *   q, out [q_rows] rows of [heads][head_dim], row strides ldq / ldo elements
+ *   k, v   [k_rows] rows of [kv_heads][head_dim], row strides ldk / ldv
+ *          (heads a multiple of kv_heads; query head h reads key/value head
+ *          h / (heads / kv_heads); q, k and v may be views of one QKV row)
+ *   q_starts [batch + 1] (device): sequence b holds query rows q_starts[b] ..
+ *          q_starts[b + 1] - 1; ascending, clamped to q_rows
+ *   k_starts the same for the key rows; NULL: q_starts (no rows before the
+ *          prompt).  With lq query and lk key rows, query row i sees keys
+ *          0 .. i + lk - lq: the queries are the sequence's last rows, as when
+ *          a prompt is run in chunks.  A row that sees no key is zero.
+ * Rows of q that no sequence holds are not written.  What other sequences'
+ * rows hold, NaN included, never reaches a sequence; a non-finite value of
+ * its own may reach every row of it, as in the reference's P . V.
+ * head_dim 32, 64 or 128.  mode (FML_MATH_*) is the precision of fp32 inputs;
+ * fp16 and bf16 products run on the tensor cores with fp32 accumulators, the
+ * probabilities rounded to the inputs' type.  Allocates nothing. */
+FML_API int fml_attention_packed(void* out, const void* q, const void* k, const void* v, int type,
+                                 const uint32_t* q_starts, const uint32_t* k_starts, uint32_t batch,
+                                 uint32_t q_rows, uint32_t k_rows, uint32_t heads, uint32_t kv_heads,
+                                 uint32_t head_dim, uint32_t ldo, uint32_t ldq, uint32_t ldk, uint32_t ldv,
+                                 float scale, int mode, fml_stream_t stream);
+
+/* The cache.  One layer's pool is [pages][kv_heads] blocks; a block holds
+ * page_size (16, 32, 64 or 128) rows of one key/value head in
+ * fml_kv4_block_bytes(head_dim, page_size) = page_size * head_dim * 5 / 4
+ * bytes: the keys' codes [page_size][head_dim / 2 bytes], the keys' pairs
+ * [page_size][head_dim / 32] of fp16 (scale, minimum), then the values' codes
+ * and pairs.  Each 32 head columns of a row are a group; a value stands for
+ * minimum + code * scale, code 0..15:
+ *   x clamped to +-65504; minimum = fp16(min x); scale = fp16((max x -
+ *   minimum) * fp32(1/15)); code = clamp(rint((x - minimum) * (1 / scale)),
+ *   0, 15), 0 where scale is 0; all in fp32, round to nearest even.  A NaN
+ *   makes its group's scale and minimum NaN.
+ * With NG = head_dim / 32, the 4-byte word of eight key codes from column
+ * 32 g + 8 c is word c * NG + g of its row, the 2-byte unit of four value
+ * codes from column 32 g + 4 n is unit n * NG + g; code i sits in bits 4 i ..
+ * 4 i + 3.  pool must be 16-byte aligned.
+ *
+ * A sequence lives in a slot: table [slots][max_pages] holds its pages in
+ * order (-1: none) and lens [slots] its rows.  refs [pages] counts the slots
+ * that hold a page (0: free).  All four are device arrays of the caller's,
+ * shared by every layer.  Entry i of a batch is slot slot_ids[i], or slot i
+ * where slot_ids is NULL.  An entry that names no slot is an empty sequence,
+ * and a table entry that names no page is a page of masked keys: the kernels
+ * never read or write outside the arrays. */
+FML_API size_t fml_kv4_block_bytes(uint32_t head_dim, uint32_t page_size);
+
+/* Writes the newest rows of each sequence: entry b's rows starts[b] ..
+ * starts[b + 1] - 1 of k and v ([rows][kv_heads][head_dim], row strides ldk /
+ * ldv) become its rows lens - n .. lens - 1 (n their number; reserve first).
+ * fml_kv4_read writes the values that the same rows stand for into k and v. */
+FML_API int fml_kv4_append(void* pool, const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids,
+                           const void* k, const void* v, int type, const uint32_t* starts, uint32_t batch,
+                           uint32_t rows, uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots,
+                           uint32_t max_pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim,
+                           fml_stream_t stream);
+FML_API int fml_kv4_read(void* k, void* v, int type, const void* pool, const int32_t* table, const uint32_t* lens,
+                         const uint32_t* slot_ids, const uint32_t* starts, uint32_t batch, uint32_t rows,
+                         uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages,
+                         uint32_t page_size, uint32_t kv_heads, uint32_t head_dim, fml_stream_t stream);
+
+/* Attention of one query row per sequence over the cache: q, out [batch] rows
+ * of [heads][head_dim], row strides ldq / ldo; entry b sees its lens keys (0
+ * gives zeros).  The key range of long sequences is split across CTAs;
+ * `workspace` (device, 16-byte aligned, any content, at least
+ * fml_attention_kv4_workspace_bytes of these sizes, 0 where nothing can be
+ * split) holds the splits' partial results until the call's kernels end. */
+FML_API size_t fml_attention_kv4_workspace_bytes(uint32_t batch, uint32_t heads, uint32_t kv_heads,
+                                                 uint32_t head_dim, uint32_t max_pages, uint32_t page_size);
+FML_API int fml_attention_kv4(void* out, const void* q, int type, uint32_t ldo, uint32_t ldq, const void* pool,
+                              const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids, uint32_t batch,
+                              uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size, uint32_t heads,
+                              uint32_t kv_heads, uint32_t head_dim, float scale, void* workspace,
+                              size_t workspace_bytes, fml_stream_t stream);
+
+/* Page operations.  They run on the device, in stream order, and take the
+ * lowest free page first, so their results do not depend on timing.  A call
+ * that cannot be carried out changes nothing but *status (device), into which
+ * it ORs why: FML_KV4_NO_PAGES, FML_KV4_BAD_SLOT (a slot out of range or
+ * named twice, or a child that holds rows), FML_KV4_ROW_FULL (a sequence
+ * longer than its table row).
+ *   reserve  lens[slot] += counts[i], with pages for the new rows
+ *   fork     slot children[i] becomes a copy of slot parents[i]: full pages
+ *            are shared (their counts rise), a page in use is copied, in
+ *            every layer, so that both may append
+ *   free     the slots' pages are given back and their lens set to 0 (a slot
+ *            named twice is freed once; one out of range is noted and skipped)
+ *   compact  with n pages in use, the i-th used page from page n on moves to
+ *            the i-th free page below n, in every layer, and the tables follow:
+ *            afterwards pages 0 .. n - 1 are the used ones
+ * The pool's layers are layer_stride bytes apart and a page has page_bytes
+ * (kv_heads blocks); both multiples of 16; at most 2^21 pages.  `workspace` (device, 16-byte
+ * aligned, any content): fml_kv4_pages_workspace_bytes(pages, n) bytes (n = 0
+ * for compact). */
+enum fml_kv4_status { FML_KV4_NO_PAGES = 1, FML_KV4_BAD_SLOT = 2, FML_KV4_ROW_FULL = 4 };
+FML_API size_t fml_kv4_pages_workspace_bytes(uint32_t pages, uint32_t n);
+FML_API int fml_kv4_reserve(int32_t* refs, int32_t* table, uint32_t* lens, const uint32_t* slot_ids,
+                            const uint32_t* counts, uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages,
+                            uint32_t page_size, int32_t* status, void* workspace, size_t workspace_bytes,
+                            fml_stream_t stream);
+FML_API int fml_kv4_fork(void* pool, uint32_t layers, uint64_t layer_stride, uint64_t page_bytes, int32_t* refs,
+                         int32_t* table, uint32_t* lens, const uint32_t* parents, const uint32_t* children,
+                         uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
+                         int32_t* status, void* workspace, size_t workspace_bytes, fml_stream_t stream);
+FML_API int fml_kv4_free(int32_t* refs, int32_t* table, uint32_t* lens, const uint32_t* slot_ids, uint32_t n,
+                         uint32_t pages, uint32_t slots, uint32_t max_pages, int32_t* status, fml_stream_t stream);
+FML_API int fml_kv4_compact(void* pool, uint32_t layers, uint64_t layer_stride, uint64_t page_bytes, int32_t* refs,
+                            int32_t* table, uint32_t pages, uint32_t slots, uint32_t max_pages, void* workspace,
+                            size_t workspace_bytes, fml_stream_t stream);
+
 /* ---------------------------------------------------------------------
  * 2. Decode engine
  * ------------------------------------------------------------------- */
