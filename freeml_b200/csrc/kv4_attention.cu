@@ -173,6 +173,17 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+// acc += a (hi + lo), the products' sum rounded into acc
+__device__ __forceinline__ void add_products(float (&acc)[4], const uint32_t (&a)[4], const uint32_t (&hi)[2],
+                                             const uint32_t (&lo)[2])
+{
+    float d[4];
+    mma_f16_zero(d, a[0], a[1], a[2], a[3], lo[0], lo[1]);
+    mma_f16(d, a, hi[0], hi[1]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] += d[x];
+}
+
 struct Segment
 {
     uint32_t b, index, of, first;  // entry, number among its `of` segments, its first segment's number
@@ -436,13 +447,14 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     const uint32_t a1[4] = {codes_low<FULL>(r0), codes_low<FULL>(r1), codes_high<FULL>(r0),
                                             codes_high<FULL>(r1)};
                     float d[4];
-                    mma_f16_zero(d, a0[0], a0[1], a0[2], a0[3], qh[g][0][0], qh[g][0][1]);
-                    mma_f16(d, a1, qh[g][1][0], qh[g][1][1]);
-                    if constexpr (FULL)
+                    if constexpr (FULL)  // the small products first
                     {
-                        mma_f16(d, a0, ql[g][0][0], ql[g][0][1]);
+                        mma_f16_zero(d, a0[0], a0[1], a0[2], a0[3], ql[g][0][0], ql[g][0][1]);
                         mma_f16(d, a1, ql[g][1][0], ql[g][1][1]);
+                        mma_f16(d, a0, qh[g][0][0], qh[g][0][1]);
                     }
+                    else mma_f16_zero(d, a0[0], a0[1], a0[2], a0[3], qh[g][0][0], qh[g][0][1]);
+                    mma_f16(d, a1, qh[g][1][0], qh[g][1][1]);
                     const float k0 = low_half(km[0][g]), k1 = low_half(km[1][g]);
                     tt[0] = fma2(make_float2(k0, k0), make_float2(d[0], d[1]), tt[0]);
                     tt[1] = fma2(make_float2(k1, k1), make_float2(d[2], d[3]), tt[1]);
@@ -559,10 +571,20 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     const float mid = FULL ? fmaf(8.f, v.x, v.y) : v.y;
                     u2[g] = fma2(p[k], make_float2(mid, mid), u2[g]);
                 }
-                mma_f16(acc[g][0], a0, hi[0], hi[1]);
-                mma_f16(acc[g][1], a1, hi[0], hi[1]);
-                mma_f16(acc[g][0], a0, lo[0], lo[1]);
-                mma_f16(acc[g][1], a1, lo[0], lo[1]);
+                if constexpr (FULL)
+                {
+                    // the tensor cores' running sums are cut, not rounded: fp32
+                    // sums of many keys are kept outside them
+                    add_products(acc[g][0], a0, hi, lo);
+                    add_products(acc[g][1], a1, hi, lo);
+                }
+                else
+                {
+                    mma_f16(acc[g][0], a0, hi[0], hi[1]);
+                    mma_f16(acc[g][1], a1, hi[0], hi[1]);
+                    mma_f16(acc[g][0], a0, lo[0], lo[1]);
+                    mma_f16(acc[g][1], a1, lo[0], lo[1]);
+                }
             }
         }
     }
