@@ -32,6 +32,7 @@
 // which a second kernel joins.
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "kv4.cuh"
 
 namespace fml {
@@ -94,26 +95,6 @@ __device__ __forceinline__ float ex2(float x)
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
-
-// two fp32 fused multiply-adds in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
-          "l"(reinterpret_cast<const uint64_t&>(c)));
-    return d;
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return d;
-}
 
 // two floats as halves, and what the halves leave of them as halves
 __device__ __forceinline__ void split2(float2 x, uint32_t* hi, uint32_t* lo)

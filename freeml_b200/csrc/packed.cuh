@@ -103,4 +103,7 @@ __device__ __forceinline__ uint32_t keys_seen(const PackedTile& p, uint32_t t)
 // Tiles at most: every sequence's last one may be part full.
 inline uint64_t packed_tiles_bound(const PackedArgs& a) { return (uint64_t)a.q_rows / a.tpt + a.batch; }
 
+int launch_packed_attention_tc(void* out, const void* q, const void* k, const void* v, int type, uint32_t head_dim,
+                               const PackedArgs& a, cudaStream_t st);
+
 }  // namespace fml

@@ -211,6 +211,11 @@ extern "C" int fml_attention_packed(void* out, const void* q, const void* k, con
     a.ldv = ldv;
     a.scale = scale;
     cudaStream_t st = as_stream(stream);
+    if (type != FML_TYPE_FP32)
+    {
+        const int rc = launch_packed_attention_tc(out, q, k, v, type, head_dim, a, st);
+        if (rc != FML_ERR_UNSUPPORTED) return rc;
+    }
     auto go = [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (head_dim == 32) return launch_simt<T, 32>(out, q, k, v, a, st);

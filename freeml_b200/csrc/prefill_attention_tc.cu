@@ -407,46 +407,6 @@ enum PpBar { PB_QF, PB_QR, PB_KF, PB_KR = PB_KF + 2, PB_KE = PB_KR + 2, PB_VF = 
 // [128, 192), Q lo [192, 256)
 constexpr uint32_t PP_TX = 256, PP_PLO = 64, PP_O = 128, PP_QLO = 192;
 
-__device__ __forceinline__ bool mbar_try(uint32_t addr, uint32_t parity)
-{
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Bounded wait for phase `ph` of `bar`; false when the limit ran out (the
-// flag is then raised) or another role raised the flag.
-__device__ __forceinline__ bool pp_wait(uint64_t* bar, uint32_t ph, volatile int* abort)
-{
-    const uint32_t addr = tc::smem_u32(bar);
-    for (uint32_t it = 0; it < (1u << 24); ++it)
-    {
-        if (mbar_try(addr, ph & 1u)) return true;
-        if ((it & 255u) == 255u && *abort) return false;
-    }
-    *abort = 1;
-    return false;
-}
-
-// 2^x by the hardware approximation (PTX ex2.approx.ftz.f32: relative error
-// about 2^-22; 2^-inf = +0)
-__device__ __forceinline__ float ex2_approx(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 }  // namespace
 
 template <bool SPLIT3>
@@ -517,7 +477,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         const uint32_t tx = tmem + PP_TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
         float m = -INFINITY, l = 0.f;
-        bool ok = __all_sync(FULL_MASK, pp_wait(&bars[PB_QF], 0, abort));
+        bool ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_QF], 0, abort));
         if (ok && SPLIT3)
         {
             // Q lo of this row into TMEM: row r of box j holds head columns
@@ -545,7 +505,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         mbar_arrive(&bars[PB_QR]);
         for (uint32_t t = 0; ok && t < nt; ++t)
         {
-            ok = __all_sync(FULL_MASK, pp_wait(&bars[PB_S0 + x], t, abort));
+            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_S0 + x], t, abort));
             if (!ok) break;
             tc_fence_after();
             float s[PP_KT];
@@ -645,7 +605,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         }
         if (ok && nt > 0)
         {
-            ok = __all_sync(FULL_MASK, pp_wait(&bars[PB_O0 + x], nt - 1, abort));
+            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_O0 + x], nt - 1, abort));
             if (ok)
             {
                 tc_fence_after();
@@ -674,7 +634,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             const uint32_t bf = t & 1u, ph = t >> 1;
             // K(t): lo rows from the hi rows the copy wrote (box j = 512
             // float4 hi, then 512 lo)
-            if (!pp_wait(&bars[PB_KF + bf], ph, abort)) break;
+            if (!mbar_wait_or(&bars[PB_KF + bf], ph, abort)) break;
             if constexpr (SPLIT3)
             {
                 // 16 loads in flight per thread before the stores
@@ -694,7 +654,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             // V(t): key block kb = hi boxes (256 float4 each) then lo boxes;
             // rows at or past `nkeys` are zeroed (the cache there may hold
             // anything, and 0 * NaN is NaN)
-            if (!pp_wait(&bars[PB_VF + bf], ph, abort)) break;
+            if (!mbar_wait_or(&bars[PB_VF + bf], ph, abort)) break;
             {
                 const uint32_t k0 = t * PP_KT;
                 const uint32_t valid = nkeys - k0 < (uint32_t)PP_KT ? nkeys - k0 : (uint32_t)PP_KT;
@@ -745,13 +705,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             const uint64_t dq = smem_desc(q_s + x * PP_QTILE, 0);
             const uint64_t dk = smem_desc(k_op, 0), dv = desc_mn(v_op);
             const uint32_t ts = tmem + PP_TX * x, to = ts + PP_O;
-            bool ok = pp_wait(&bars[PB_QR], 0, abort);
+            bool ok = mbar_wait_or(&bars[PB_QR], 0, abort);
             for (uint32_t t = 0; ok && t < nt; ++t)
             {
                 const uint32_t bf = t & 1u, ph = t >> 1;
                 // S_x(t) = Q_x K(t)^T, after O_x(t-1) has read P_x(t-1)
-                if (!(ok = pp_wait(&bars[PB_KR + bf], ph, abort))) break;
-                if (t > 0 && !(ok = pp_wait(&bars[PB_O0 + x], t - 1, abort))) break;
+                if (!(ok = mbar_wait_or(&bars[PB_KR + bf], ph, abort))) break;
+                if (t > 0 && !(ok = mbar_wait_or(&bars[PB_O0 + x], t - 1, abort))) break;
                 tc_fence_after();
                 const uint64_t kbase = dk + ((bf * PP_KVOP) >> 4);
 #pragma unroll
@@ -773,8 +733,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 mma_commit(&bars[PB_S0 + x]);
                 mma_commit(&bars[PB_KE + 2 * x + bf]);
                 // O_x += P_x(t) V(t)
-                if (!(ok = pp_wait(&bars[PB_VR + bf], ph, abort))) break;
-                if (!(ok = pp_wait(&bars[PB_P0 + x], t, abort))) break;
+                if (!(ok = mbar_wait_or(&bars[PB_VR + bf], ph, abort))) break;
+                if (!(ok = mbar_wait_or(&bars[PB_P0 + x], t, abort))) break;
                 tc_fence_after();
                 const uint64_t vbase = dv + ((bf * PP_KVOP) >> 4);
 #pragma unroll
@@ -815,15 +775,15 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             {
                 const uint32_t bf = t & 1u;
                 // K(t) into buffer t % 2 once S_A(t-2) and S_B(t-2) have read it
-                if (t >= 2 && t - 2 < nt0 && !pp_wait(&bars[PB_KE + bf], (t >> 1) - 1, abort)) break;
-                if (t >= 2 && t - 2 < nt1 && !pp_wait(&bars[PB_KE + 2 + bf], (t >> 1) - 1, abort)) break;
+                if (t >= 2 && t - 2 < nt0 && !mbar_wait_or(&bars[PB_KE + bf], (t >> 1) - 1, abort)) break;
+                if (t >= 2 && t - 2 < nt1 && !mbar_wait_or(&bars[PB_KE + 2 + bf], (t >> 1) - 1, abort)) break;
                 mbar_arrive_expect_tx(&bars[PB_KF + bf], PP_KVT);
                 for (int j = 0; j < PP_HD / 32; ++j)
                     tma_load_2d(k_op + bf * PP_KVOP + j * PP_KBOX, &map_k, 32 * j, kv_row0 + (int)(t * PP_KT),
                                 &bars[PB_KF + bf]);
                 // V(t) once O_A(t-2) and O_B(t-2) have
-                if ((t >= 2 && t - 2 < nt0 && !pp_wait(&bars[PB_VE + bf], (t >> 1) - 1, abort)) ||
-                    (t >= 2 && t - 2 < nt1 && !pp_wait(&bars[PB_VE + 2 + bf], (t >> 1) - 1, abort)))
+                if ((t >= 2 && t - 2 < nt0 && !mbar_wait_or(&bars[PB_VE + bf], (t >> 1) - 1, abort)) ||
+                    (t >= 2 && t - 2 < nt1 && !mbar_wait_or(&bars[PB_VE + 2 + bf], (t >> 1) - 1, abort)))
                 {
                     issued = 2 * t + 1;
                     break;

@@ -88,6 +88,21 @@ def test_prompts(kind, heads, kv, hd, lens):
 
 
 @pytest.mark.parametrize("kind", sorted(DT))
+@pytest.mark.parametrize("heads,kv,hd", [(4, 4, 32), (2, 1, 64), (4, 1, 128)])
+@pytest.mark.parametrize("n", [1280, 1537, 2300, 4095])
+def test_many_key_tiles(kind, heads, kv, hd, n):
+    """Every stage of the copies' ring is used more than once, and the last key
+    tile is whole, or ends inside the sequence's last rows."""
+    lq, lk = [n, 60, 130], [n, n + 60, n + 130]
+    q, k, v = make(lq, lk, heads, kv, hd, kind, 9)
+    v[n + n + 60:][:n] += 1.0
+    out = torch.full_like(q, float("nan"))
+    scale = 1.0 / math.sqrt(hd)
+    matrix_ops.attention_packed(out, q, k, v, starts_of(lq), scale, k_starts=starts_of(lk))
+    check(out, *reference(q, k, v, lq, lk, scale, kind))
+
+
+@pytest.mark.parametrize("kind", sorted(DT))
 @pytest.mark.parametrize("heads,kv,hd", [(4, 4, 64), (8, 2, 128), (4, 1, 32)])
 def test_keys_lead_or_lag_the_queries(kind, heads, kv, hd):
     """Chunks after a prefix; and sequences with fewer keys than rows, whose
@@ -216,6 +231,13 @@ def test_many_sequences_and_a_stream_of_its_own():
     again = torch.empty_like(q)
     matrix_ops.attention_packed(again, q, k, v, starts, 0.2)
     assert torch.equal(out, again)
+
+
+def test_no_wait_ran_out():
+    import ctypes
+    n = ctypes.c_uint64(1)
+    _lib.call("fml_device_error_count", ctypes.byref(n))
+    assert n.value == 0
 
 
 def test_refusals():
