@@ -8,21 +8,27 @@
 // phases interleave: the tensor cores work on one while the other's softmax
 // runs.
 //   warps 0-3, 4-7  softmax of tile A, B (thread = TMEM lane = query row)
-//   warps 8, 9      one thread each issues tile A's / B's tcgen05.mma
+//   warps 8, 9      tile A's / B's tcgen05.mma (one lane elected)
 //   warp 10         one thread issues every TMA copy; the warp then zeroes the
 //                   rows past the sequence's end in its last value tile
 //                   (another sequence's rows, or its NaN, lie there)
 //   warp 11         idle: registers are shared out by groups of four warps
-// Key and value tiles have 128 rows.  TMEM, per query tile: S (128 fp32
-// columns), overwritten in place by P in 16 bits (64 columns, the A operand of
-// O += P V, read from TMEM), and the output's hd columns, which stay there
-// over all key tiles.  A row rescales its output only when its running maximum
-// rises by more than 2^8 over the one its P was taken against; fp16 P is taken
-// 2^7 larger, so that it uses the type's range (at most 2^15) and small
+// Keys and values are copied 128 rows at a time and used in halves of 64.  TMEM,
+// per query tile: two score buffers of 64 fp32 columns, S of half i in buffer
+// i % 2, overwritten in place by P in 16 bits (32 columns, the A operand of
+// O += P V, read from TMEM), and the output's hd columns, which stay there over
+// all keys.  With two buffers S of half i + 1 is there before P of half i is, and
+// the softmax warps never wait for a product in the steady state; one buffer of
+// 128 keys costs the tensor cores less (an S product of 64 keys takes 3/4 of the
+// time of one of 128) but took 4640 cycles for 128 keys and 256 rows of head
+// dim 128, against 3950.
+// A row rescales its output only when a score rises by more than 2^8 (bf16:
+// 2^40) over the maximum that its P is taken against; fp16 P is taken 2^7
+// larger, so that it uses the type's range (at most 2^15) and small
 // probabilities stay above its smallest numbers.
 //
 // What bounds it: per 128 keys and 256 rows of head dim 128, the products take
-// 2048 cycles of the tensor cores and the exponentials 2048 of the special
+// 2560 cycles of the tensor cores and the exponentials 2048 of the special
 // function units.
 // Every wait is bounded and returns early once any role has recorded an expiry.
 #include <cuda_bf16.h>
@@ -41,7 +47,8 @@ __device__ int g_packed_tc_timeouts;
 namespace {
 
 constexpr int THREADS = 12 * 32;
-constexpr int KT = 128;  // keys of a tile
+constexpr int KT = 128;  // keys of a copied tile
+constexpr int KH = 64;   // keys of a half: one S and one P product
 
 template <int HD>
 struct Shape
@@ -53,8 +60,8 @@ struct Shape
     static constexpr uint32_t TILE = BOXES * BOX;       // a Q, K or V tile
     static constexpr int STAGES = HD == 128 ? 2 : 4;
     static constexpr uint32_t SMEM = 2 * TILE + 2 * STAGES * TILE + 1024 + 512;
-    // TMEM columns: S / P and the output of tile x
-    static constexpr uint32_t TX = 256, O = 128;
+    // TMEM columns of tile x: S / P buffers 0 and 1, the output
+    static constexpr uint32_t TX = 256, O = 2 * KH;
     // shared-memory operand descriptors: 8-row groups of the swizzled rows
     static constexpr uint64_t LAYOUT = HD < 64 ? 4ull << 61 : 2ull << 61;  // 64- or 128-byte swizzle
     static constexpr uint64_t SBO = (uint64_t)(8 * ROW >> 4) << 32;
@@ -63,8 +70,9 @@ struct Shape
     static constexpr uint64_t VDESC = LAYOUT | SBO | ((uint64_t)(BOX >> 4) << 16) | (1ull << 46);
 };
 
-enum Bar { B_QF, B_VR, B_S0, B_P0 = B_S0 + 2, B_O0 = B_P0 + 2, B_FIN = B_O0 + 2, B_KF = B_FIN + 2 };
-// then, per stage: K and V copies landed, K and V of each query tile consumed
+// per query tile x: S and P by buffer (2 x + buffer), the output, the end; per
+// stage: K and V copies landed, K and V consumed by each query tile
+enum Bar { B_QF, B_VR, B_S0, B_P0 = B_S0 + 4, B_O0 = B_P0 + 4, B_FIN = B_O0 + 2, B_KF = B_FIN + 2 };
 template <int ST>
 struct Bars
 {
@@ -78,12 +86,17 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N)
     return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// Products and commits are issued by a whole warp, of which the hardware elects
+// one lane: its operands are then the same in the warp for the compiler too.
+// From a branch of one thread a product costs 80 to 130 cycles to issue, more
+// than it takes; so, 15 to 25.
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
@@ -91,10 +104,20 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, u
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void commit(uint64_t* bar)
+{
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar))
         : "memory");
 }
 
@@ -105,6 +128,23 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         "[%5];" ::"r"(tc::smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
         : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Scores `first` .. of 32 columns, where a mask bites, to -inf (a select: NaN may lie there).
+__device__ __forceinline__ void mask32(uint32_t (&u)[32], bool masked, int first)
+{
+    if (masked)
+    {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) u[i] = i < first ? u[i] : 0xff800000u;
+    }
 }
 
 template <typename T>
@@ -134,7 +174,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     using Sh = Shape<HD>;
     constexpr int ST = Sh::STAGES;
     using Bx = Bars<ST>;
-    constexpr uint32_t IDESC_S = idesc_f16<T>(128, KT);
+    constexpr uint32_t IDESC_S = idesc_f16<T>(128, KH);
     constexpr uint32_t IDESC_O = idesc_f16<T>(128, HD) | (1u << 16);  // values read N-major
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem =
@@ -156,17 +196,17 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     const uint32_t nh = min(a.gs, a.group - hc);                        // query heads of the tiles
     const uint32_t tokens = min(pair.tpt, p.lq - p.t0);
     const uint32_t tok0 = min(a.tpt, tokens), tok1 = tokens - tok0;     // tokens of tile A, B
-    // key tiles of tile A and B
-    const uint32_t nt0 = (keys_seen(p, p.t0 + tok0 - 1) + KT - 1) / KT;
-    const uint32_t nt1 = tok1 ? (keys_seen(p, p.t0 + tokens - 1) + KT - 1) / KT : 0u;
-    const uint32_t ntiles = max(nt0, nt1);
+    // halves of tile A and B, and the key tiles that hold them
+    const uint32_t n0 = (keys_seen(p, p.t0 + tok0 - 1) + KH - 1) / KH;
+    const uint32_t n1 = tok1 ? (keys_seen(p, p.t0 + tokens - 1) + KH - 1) / KH : 0u;
+    const uint32_t nt0 = (n0 + 1) / 2, nt1 = (n1 + 1) / 2, ntiles = max(nt0, nt1);
     // keys of the last tile that are the sequence's
     const uint32_t tail = ntiles ? min((uint32_t)KT, p.lk - (ntiles - 1) * KT) : (uint32_t)KT;
 
     if (tid == 0)
     {
         for (int i = 0; i < Bx::N; ++i)
-            mbar_init(&bars[i], i == B_VR ? 32u : i == B_P0 || i == B_P0 + 1 ? 128u : 1u);
+            mbar_init(&bars[i], i == B_VR ? 32u : i >= B_P0 && i < B_P0 + 4 ? 128u : 1u);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -190,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     {
         // ---------------- softmax of tile x ----------------
         const int x = warp >> 2;
-        const uint32_t nt = x ? nt1 : nt0;
+        const uint32_t n = x ? n1 : n0;
         const uint32_t r = 32 * (warp & 3) + lane, tok = r / a.gs, head = r % a.gs;
         const bool live = tok < (x ? tok1 : tok0) && head < nh;
         const uint32_t token = p.t0 + (x ? a.tpt : 0u) + tok;
@@ -198,94 +238,95 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
         const uint32_t seen = live ? keys_seen(p, token) : 0xffffffffu;
         const uint32_t least = __reduce_min_sync(FULL_MASK, seen);
         const uint32_t tx = tmem + Sh::TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
-        constexpr float LIFT = std::is_same_v<T, __half> ? 7.f : 0.f;
+        // P is 2^(s - m + LIFT), at most 2^(RISE + LIFT): bf16 has fp32's range
+        constexpr float LIFT = std::is_same_v<T, __half> ? 7.f : 0.f, RISE = std::is_same_v<T, __half> ? 8.f : 40.f;
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units; scale > 0
         float m = -INFINITY;  // running maximum, in log2 units
         float2 l2 = make_float2(0.f, 0.f);
         bool ok = true;
-        for (uint32_t t = 0; t < nt; ++t)
+        for (uint32_t i = 0; i < n; ++i)
         {
-            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_S0 + x], t, abort));
+            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_S0 + 2 * x + (i & 1u)], i >> 1, abort));
             if (!ok) break;
             tc_fence_after();
-            float s[KT];
+            const uint32_t k0 = i * KH, ts = tx + KH * (i & 1u);
+            const bool masked = k0 + KH > least;  // the same in the whole warp
+            const int reach = (int)min(seen - k0, (uint32_t)KH) * (seen > k0);  // keys of this half that the row sees
+            // P against the maximum so far; where a row's maximum has risen too
+            // far, its output is rescaled and P computed again (as is the first)
+            uint32_t w[32];
+            float2 sum;
+            while (true)
             {
-                uint32_t u[4][32];
+                const float base = m == -INFINITY ? 0.f : LIFT - m;  // no key yet: 2^(-inf) = 0
+                const float2 scale2 = make_float2(sl2, sl2), base2 = make_float2(base, base);
+                uint32_t u[2][32];
+                tmem_ld32_async(ts, u[0]);
+                tmem_ld32_async(ts + 32, u[1]);
+                sum = make_float2(0.f, 0.f);
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_wait_ld(u[0]);
+                tmem_wait_ld(u[1]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_async(tx + 32 * c, u[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c)
                 {
-                    tmem_wait_ld(u[c]);
+                    mask32(u[c], masked, reach - 32 * c);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[32 * c + i] = __uint_as_float(u[c][i]);
+                    for (int j = 0; j < 16; ++j)
+                    {
+                        const float s0 = __uint_as_float(u[c][2 * j]), s1 = __uint_as_float(u[c][2 * j + 1]);
+                        mx[j & 3] = max3(mx[j & 3], s0, s1);
+                        const float2 e = fma2(make_float2(s0, s1), scale2, base2);
+                        const float2 q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                        sum = add2(sum, q);
+                        w[16 * c + j] = pack2<T>(q.x, q.y);
+                    }
                 }
-            }
-            const uint32_t k0 = t * KT;
-            if (k0 + KT > least)
-            {
-#pragma unroll
-                for (int i = 0; i < KT; ++i) s[i] = k0 + i < seen ? s[i] : -INFINITY;  // a select: NaN may lie there
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < KT; i += 8)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], fmaxf(s[i + 2 * j], s[i + 2 * j + 1]));
-            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-            const bool need = mt > m + 8.0f;
-            if (__any_sync(FULL_MASK, need))
-            {
+                const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
+                const bool need = mt > m + RISE;
+                if (!__any_sync(FULL_MASK, need)) break;
                 const float mn = need ? mt : m;
                 const float corr = need ? ex2_approx(m - mn) : 1.0f;
                 l2.x *= corr;
                 l2.y *= corr;
                 m = mn;
-                if (t > 0)
+                if (i > 0)
                 {
-                    // O_x(t-1) has completed: S_x(t) was issued after it
+                    // the product of half i - 1 must have gone into the output
+                    // (that of i - 2 has: S of half i was issued after it)
+                    if (!(ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_O0 + x], i - 1, abort)))) break;
+                    tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < HD; c += 32)
                     {
                         float v[32];
-                        uint32_t u[32];
+                        uint32_t o[32];
                         tmem_ld32(tx + Sh::O + c, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * corr);
-                        tmem_st32(tx + Sh::O + c, u);
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j] * corr);
+                        tmem_st32(tx + Sh::O + c, o);
                     }
                 }
             }
-            const float base = m == -INFINITY ? 0.f : LIFT - m;  // no key yet: 2^(-inf) = 0
-            const float2 scale2 = make_float2(sl2, sl2), base2 = make_float2(base, base);
-#pragma unroll
-            for (int c = 0; c < KT; c += 64)
-            {
-                uint32_t u[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                {
-                    const float2 e = fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), scale2, base2);
-                    const float2 q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                    l2 = add2(l2, q);
-                    u[i] = pack2<T>(q.x, q.y);
-                }
-                tmem_st32(tx + c / 2, u);
-            }
+            if (!ok) break;
+            l2 = add2(l2, sum);
+            tmem_st32(ts, w);  // over scores that have been read
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&bars[B_P0 + x]);
+            mbar_arrive(&bars[B_P0 + 2 * x + (i & 1u)]);
         }
-        if (ok && nt > 0)
+        if (ok && n > 0)
         {
-            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_O0 + x], nt - 1, abort));
+            // every product of the tile is done (a barrier of one phase: this
+            // thread has not followed the output's, and may be two behind)
+            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_FIN + x], 0, abort));
             tc_fence_after();
         }
         if (ok)
         {
             const float l = l2.x + l2.y, inv = l == 0.f ? 0.f : 1.0f / l;
             T* dst = out + (uint64_t)(p.q0 + token) * a.ldo + (uint64_t)(kvh * a.group + hc + head) * HD;
-            if (nt == 0)
+            if (n == 0)
             {
                 if (live)
                     for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
@@ -310,20 +351,18 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     {
         // ---------------- MMA issue for tile x ----------------
         const int x = warp - 8;
-        const uint32_t nt = x ? nt1 : nt0;
-        if (lane == 0 && nt > 0)
+        const uint32_t n = x ? n1 : n0;
+        if (n > 0)
         {
+            auto wait = [&](int b, uint32_t ph) { return __all_sync(FULL_MASK, mbar_wait_or(&bars[b], ph, abort)); };
             const uint64_t dq = Sh::KDESC | (uint64_t)(smem_u32(q_s + x * Sh::TILE) >> 4);
             const uint64_t dk = Sh::KDESC | (uint64_t)(smem_u32(k_s) >> 4);
             const uint64_t dv = Sh::VDESC | (uint64_t)(smem_u32(v_s) >> 4);
             const uint32_t ts = tmem + Sh::TX * x, to = ts + Sh::O;
-            bool ok = mbar_wait_or(&bars[B_QF], 0, abort);
-            for (uint32_t t = 0; ok && t < nt; ++t)
-            {
-                const uint32_t st = t % ST, ph = t / ST;
-                // S_x(t), after O_x(t-1) has read P_x(t-1)
-                if (!(ok = mbar_wait_or(&bars[Bx::KF + st], ph, abort))) break;
-                if (t > 0 && !(ok = mbar_wait_or(&bars[B_O0 + x], t - 1, abort))) break;
+            // S of half i into its buffer; the last half of a key tile frees it
+            auto scores = [&](uint32_t i) {
+                const uint32_t st = (i >> 1) % ST, buf = i & 1u;
+                const uint64_t kb = dk + ((st * Sh::TILE + buf * KH * Sh::ROW) >> 4);
                 tc_fence_after();
 #pragma unroll
                 for (int j = 0; j < Sh::BOXES; ++j)
@@ -331,24 +370,42 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
                     for (int kk = 0; kk < Sh::COLS / 16; ++kk)
                     {
                         const uint32_t off = (j * Sh::BOX + kk * 32) >> 4;
-                        mma_f16_ss(ts, dq + off, dk + ((st * Sh::TILE) >> 4) + off, IDESC_S, j > 0 || kk > 0);
+                        mma_f16_ss(ts + KH * buf, dq + off, kb + off, IDESC_S, j > 0 || kk > 0);
                     }
-                mma_commit(&bars[B_S0 + x]);
-                mma_commit(&bars[Bx::KE + ST * x + st]);
-                // O_x += P_x(t) V(t)
-                if (!(ok = mbar_wait_or(&bars[Bx::VF + st], ph, abort))) break;
-                if (t == ntiles - 1 && tail < KT && !(ok = mbar_wait_or(&bars[B_VR], 0, abort))) break;
-                if (!(ok = mbar_wait_or(&bars[B_P0 + x], t, abort))) break;
+                commit(&bars[B_S0 + 2 * x + buf]);
+                if (buf || i + 1 == n) commit(&bars[Bx::KE + ST * x + st]);
+            };
+            bool ok = wait(B_QF, 0) && wait(Bx::KF, 0);
+            if (ok) scores(0);
+            if (ok && n > 1) scores(1);
+            for (uint32_t i = 0; ok && i < n; ++i)
+            {
+                const uint32_t t = i >> 1, st = t % ST, buf = i & 1u;
+                if (!buf)
+                {
+                    if (!(ok = wait(Bx::VF + st, t / ST))) break;
+                    if (t == ntiles - 1 && tail < KT && !(ok = wait(B_VR, 0))) break;
+                }
+                // O += P V of half i
+                if (!(ok = wait(B_P0 + 2 * x + buf, t))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk)
-                    mma_f16_ts(to, ts + 8 * kk, dv + ((st * Sh::TILE + kk * 16 * Sh::ROW) >> 4), IDESC_O, t > 0 || kk > 0);
-                mma_commit(&bars[B_O0 + x]);
-                mma_commit(&bars[Bx::VE + ST * x + st]);
+                for (int kk = 0; kk < KH / 16; ++kk)
+                    mma_f16_ts(to, ts + KH * buf + 8 * kk, dv + ((st * Sh::TILE + (buf * KH + kk * 16) * Sh::ROW) >> 4),
+                               IDESC_O, i > 0 || kk > 0);
+                commit(&bars[B_O0 + x]);
+                if (buf || i + 1 == n) commit(&bars[Bx::VE + ST * x + st]);
+                if (i + 2 < n)
+                {
+                    // S of half i + 2, once P of half i, in the same buffer, has been read
+                    if (!buf && !(ok = wait(Bx::KF + (t + 1) % ST, (t + 1) / ST))) break;
+                    if (!(ok = wait(B_O0 + x, i))) break;
+                    scores(i + 2);
+                }
             }
-            // every MMA this thread issued completes before TMEM is freed
-            mma_commit(&bars[B_FIN + x]);
-            mbar_wait(&bars[B_FIN + x], 0);
+            // every MMA this warp issued completes before TMEM is freed
+            commit(&bars[B_FIN + x]);
+            __all_sync(FULL_MASK, mbar_wait(&bars[B_FIN + x], 0));
         }
     }
     else if (warp == 10)
