@@ -93,6 +93,44 @@ __device__ PackedTile packed_tile(const PackedArgs& a, uint32_t idx)
     return tile_s;
 }
 
+// The tile of number `idx` of all tiles, sequence after sequence, each from its
+// last tile to its first; called by a whole warp.
+__device__ inline PackedTile packed_tile_warp(const PackedArgs& a, uint32_t idx)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    PackedTile t{};
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 32)
+    {
+        const uint32_t b = b0 + lane;
+        uint32_t q0 = 0, n = 0, lq = 0;
+        if (b < a.batch)
+        {
+            lq = clamped_rows(a.q_starts, b, a.q_rows, &q0);
+            n = (lq + a.tpt - 1) / a.tpt;
+        }
+        uint32_t x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+        {
+            const uint32_t y = __shfl_up_sync(FULL_MASK, x, o);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        const uint32_t found = __ballot_sync(FULL_MASK, idx < x);
+        if (found)
+        {
+            const int src = __ffs(found) - 1;
+            t.q0 = __shfl_sync(FULL_MASK, q0, src);
+            t.lq = __shfl_sync(FULL_MASK, lq, src);
+            t.t0 = (__shfl_sync(FULL_MASK, x, src) - 1 - idx) * a.tpt;
+            t.lk = clamped_rows(a.k_starts, b0 + (uint32_t)src, a.k_rows, &t.k0);
+            t.live = 1;
+            return t;
+        }
+        idx -= __shfl_sync(FULL_MASK, x, 31);
+    }
+    return t;
+}
+
 // Keys that the tile's token t sees.
 __device__ __forceinline__ uint32_t keys_seen(const PackedTile& p, uint32_t t)
 {

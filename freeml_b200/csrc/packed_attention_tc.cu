@@ -2,39 +2,52 @@
 // the tensor cores: S = Q K^T * scale with the causal mask, row softmax, P V,
 // as one pass over the keys with a running maximum and sum.
 //
-// CTA = 12 warps on two tiles, A and B, of 128 query rows of one key/value
-// head (packed.cuh: tokens in order and, for each, the query heads of the
-// group, so that a group shares every key and value tile).  The two tiles'
-// phases interleave: the tensor cores work on one while the other's softmax
-// runs.
+// A CTA stays on its SM and takes one work item after another: two tiles, A and
+// B, of 128 query rows of one key/value head (packed.cuh: tokens in order and,
+// for each, the query heads of the group, so that a group shares every key and
+// value tile).  The grid has a block for every item; a running CTA takes over
+// blocks that have not started (cluster launch control), so that items of very
+// different lengths even out and barriers, TMEM and registers are set up once.
 //   warps 0-3, 4-7  softmax of tile A, B (thread = TMEM lane = query row)
-//   warps 8, 9      tile A's / B's tcgen05.mma (one lane elected)
-//   warp 10         one thread issues every TMA copy; the warp then zeroes the
-//                   rows past the sequence's end in its last value tile
-//                   (another sequence's rows, or its NaN, lie there)
-//   warp 11         idle: registers are shared out by groups of four warps
+//   warps 8, 9      issue tile A's / B's S products (tcgen05.mma, one lane elected)
+//   warps 10, 11    issue their P V products
+//   warp 12         issues every TMA copy and zeroes the rows past the
+//                   sequence's end in its last value tile (another sequence's
+//                   rows, or its NaN, lie there)
+//   warp 13         finds the next item (14 and 15 are idle: registers are
+//                   shared out by groups of four warps)
+// Each role runs ahead into the next item as far as its barriers let it: its
+// queries are copied while the last products of this one run, its first scores
+// are there when the softmax warps have written this one's output.
 // Keys and values are copied 128 rows at a time and used in halves of 64.  TMEM,
 // per query tile: two score buffers of 64 fp32 columns, S of half i in buffer
 // i % 2, overwritten in place by P in 16 bits (32 columns, the A operand of
 // O += P V, read from TMEM), and the output's hd columns, which stay there over
 // all keys.  With two buffers S of half i + 1 is there before P of half i is, and
-// the softmax warps never wait for a product in the steady state; one buffer of
-// 128 keys costs the tensor cores less (an S product of 64 keys takes 3/4 of the
-// time of one of 128) but took 4640 cycles for 128 keys and 256 rows of head
-// dim 128, against 3950.
+// the softmax warps never wait for a product in the steady state (one buffer of
+// 128 keys, whose S product costs the tensor cores less, was slower: S, softmax
+// and P V then follow one another).
 // A row rescales its output only when a score rises by more than 2^8 (bf16:
 // 2^40) over the maximum that its P is taken against; fp16 P is taken 2^7
 // larger, so that it uses the type's range (at most 2^15) and small
 // probabilities stay above its smallest numbers.
 //
-// What bounds it: per 128 keys and 256 rows of head dim 128, the products take
-// 2560 cycles of the tensor cores and the exponentials 2048 of the special
-// function units.
+// What bounds it: a half of 64 keys of both tiles takes about 2050 cycles in head
+// dim 128, of which the tensor cores work 1280 (S of 64 keys takes 3/4 of the
+// time of one of 128: shared memory's rate) and the special function units 1024.
+// The softmax warps, one of each tile to a scheduler, are what the rest waits
+// for: wait, ld, maximum, exponentials and st follow one another.  Tried and not
+// faster: four softmax warps a scheduler (a half's latency then bounds the two
+// buffers), turns at the exponentials, polynomials for a part of them.
+// Grouped bf16 prompts of up to 4096 (2.1e11 flops) take 277 us, 0.76 PFLOP/s.
 // Every wait is bounded and returns early once any role has recorded an expiry.
+// A wait tells neighbouring phases of a barrier apart only, so every role that
+// waits on a barrier follows all of its phases, or is never two behind.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <cuda/ptx>
 
 #include "f32x2.cuh"
 #include "packed.cuh"
@@ -46,7 +59,7 @@ __device__ int g_packed_tc_timeouts;
 
 namespace {
 
-constexpr int THREADS = 12 * 32;
+constexpr int THREADS = 16 * 32;
 constexpr int KT = 128;  // keys of a copied tile
 constexpr int KH = 64;   // keys of a half: one S and one P product
 
@@ -59,7 +72,7 @@ struct Shape
     static constexpr uint32_t BOX = 128 * ROW;          // 128 rows of a box
     static constexpr uint32_t TILE = BOXES * BOX;       // a Q, K or V tile
     static constexpr int STAGES = HD == 128 ? 2 : 4;
-    static constexpr uint32_t SMEM = 2 * TILE + 2 * STAGES * TILE + 1024 + 512;
+    static constexpr uint32_t SMEM = 2 * TILE + 2 * STAGES * TILE + 1024 + 1024 + 8 * 2048;
     // TMEM columns of tile x: S / P buffers 0 and 1, the output
     static constexpr uint32_t TX = 256, O = 2 * KH;
     // shared-memory operand descriptors: 8-row groups of the swizzled rows
@@ -70,13 +83,36 @@ struct Shape
     static constexpr uint64_t VDESC = LAYOUT | SBO | ((uint64_t)(BOX >> 4) << 16) | (1ull << 46);
 };
 
-// per query tile x: S and P by buffer (2 x + buffer), the output, the end; per
-// stage: K and V copies landed, K and V consumed by each query tile
-enum Bar { B_QF, B_VR, B_S0, B_P0 = B_S0 + 4, B_O0 = B_P0 + 4, B_FIN = B_O0 + 2, B_KF = B_FIN + 2 };
+// Items: found and taken (two slots), queries landed and consumed, the launch
+// control's answer.  Per query tile x: S, P and P V by buffer (2 x + buffer), the
+// item's output done and read, the end of both issuing warps.  Per stage: K and V
+// copies landed, rows past a sequence's end zeroed, K and V consumed by both
+// query tiles.
+enum Bar { B_TF, B_TE = B_TF + 2, B_QF = B_TE + 2, B_QE, B_CL, B_S0, B_P0 = B_S0 + 4, B_O0 = B_P0 + 4,
+           B_OD = B_O0 + 4, B_OE = B_OD + 2, B_FIN = B_OE + 2, B_KF = B_FIN + 4 };
 template <int ST>
 struct Bars
 {
-    static constexpr int KF = B_KF, VF = KF + ST, KE = VF + ST, VE = KE + 2 * ST, N = VE + 2 * ST;
+    static constexpr int KF = B_KF, VF = KF + ST, VR = VF + ST, KE = VR + ST, VE = KE + ST, N = VE + ST;
+    __device__ static constexpr uint32_t arrivals(int i)
+    {
+        if (i == B_TE || i == B_TE + 1) return 13;  // 8 softmax, 4 MMA warps, the copying one
+        if (i == B_QE || (i >= KE && i < N)) return 2;  // both query tiles' MMA warps
+        if (i >= VR && i < KE) return 32;
+        if ((i >= B_P0 && i < B_P0 + 4) || i == B_OE || i == B_OE + 1) return 128;
+        return 1;
+    }
+};
+
+// A work item, as the finder leaves it for the others.
+struct Item
+{
+    PackedTile p;        // live 0: no more
+    uint32_t kvh, hc;    // key/value head, first query head of the group
+    uint32_t tok0, tok1; // tokens of tile A, B
+    uint32_t n0, n1;     // halves of their keys
+    uint32_t ntiles;     // key tiles that hold them
+    uint32_t tail;       // keys of the last tile that are the sequence's
 };
 
 template <typename T>
@@ -129,6 +165,10 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
         : "memory");
 }
+
+// A value that is the same in the whole warp, as the compiler cannot see: an
+// operand of it then needs no loop over the lanes' values.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(FULL_MASK, x, 0); }
 
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
@@ -183,30 +223,17 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     unsigned char* k_s = q_s + 2 * Sh::TILE;      // stage s at s * TILE
     unsigned char* v_s = k_s + ST * Sh::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + ST * Sh::TILE);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Bx::N);
+    uint4* answer = reinterpret_cast<uint4*>(bars + (Bx::N + 1) / 2 * 2);  // of the launch control
+    Item* items = reinterpret_cast<Item*>(answer + 1);                    // two slots
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint4* staging = reinterpret_cast<uint4*>(v_s + ST * Sh::TILE + 1024);  // 2 KB a softmax warp
+    static_assert((Bx::N + 1) / 2 * 16 + 16 + 2 * sizeof(Item) + 8 <= 1024, "the barriers' room");
 
-    const uint32_t ny = a.kv_heads * a.nchunk, y = blockIdx.x % ny;
-    PackedArgs pair = a;  // a CTA has two tiles of a.tpt tokens
-    pair.tpt = 2 * a.tpt;
-    const PackedTile p = packed_tile<THREADS>(pair, blockIdx.x / ny);
-    if (!p.live) return;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t kvh = y / a.nchunk, hc = (y % a.nchunk) * a.gs;
-    const uint32_t nh = min(a.gs, a.group - hc);                        // query heads of the tiles
-    const uint32_t tokens = min(pair.tpt, p.lq - p.t0);
-    const uint32_t tok0 = min(a.tpt, tokens), tok1 = tokens - tok0;     // tokens of tile A, B
-    // halves of tile A and B, and the key tiles that hold them
-    const uint32_t n0 = (keys_seen(p, p.t0 + tok0 - 1) + KH - 1) / KH;
-    const uint32_t n1 = tok1 ? (keys_seen(p, p.t0 + tokens - 1) + KH - 1) / KH : 0u;
-    const uint32_t nt0 = (n0 + 1) / 2, nt1 = (n1 + 1) / 2, ntiles = max(nt0, nt1);
-    // keys of the last tile that are the sequence's
-    const uint32_t tail = ntiles ? min((uint32_t)KT, p.lk - (ntiles - 1) * KT) : (uint32_t)KT;
-
+    const int tid = threadIdx.x, warp = (int)uniform(tid >> 5), lane = tid & 31;
     if (tid == 0)
     {
-        for (int i = 0; i < Bx::N; ++i)
-            mbar_init(&bars[i], i == B_VR ? 32u : i >= B_P0 && i < B_P0 + 4 ? 128u : 1u);
+        for (int i = 0; i < Bx::N; ++i) mbar_init(&bars[i], Bx::arrivals(i));
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -220,257 +247,371 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
+    // a bounded wait of the whole warp
+    auto wait = [&](int b, uint32_t ph) { return __all_sync(FULL_MASK, mbar_wait_or(&bars[b], ph, abort)) != 0; };
+    // item k, once it is there (false: a wait has expired); its slot given back
+    auto take = [&](uint32_t k, Item* it) {
+        if (!wait(B_TF + (k & 1u), k >> 1)) return false;
+        *it = items[k & 1u];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[B_TE + (k & 1u)]);
+        return it->p.live != 0;
+    };
 
-    // Registers: launched with 384 x 168; a softmax thread holds a row of 128
-    // scores (2 x 128 x 208 + 128 x 80 fit the launch's)
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    // Registers: launched with 512 x 128, shared out as 2 x 128 x 192 for the
+    // softmax warps and 2 x 128 x 64
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < 8)
     {
         // ---------------- softmax of tile x ----------------
         const int x = warp >> 2;
-        const uint32_t n = x ? n1 : n0;
         const uint32_t r = 32 * (warp & 3) + lane, tok = r / a.gs, head = r % a.gs;
-        const bool live = tok < (x ? tok1 : tok0) && head < nh;
-        const uint32_t token = p.t0 + (x ? a.tpt : 0u) + tok;
-        // keys the row sees; rows that are no query's are left unmasked
-        const uint32_t seen = live ? keys_seen(p, token) : 0xffffffffu;
-        const uint32_t least = __reduce_min_sync(FULL_MASK, seen);
         const uint32_t tx = tmem + Sh::TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
         // P is 2^(s - m + LIFT), at most 2^(RISE + LIFT): bf16 has fp32's range
         constexpr float LIFT = std::is_same_v<T, __half> ? 7.f : 0.f, RISE = std::is_same_v<T, __half> ? 8.f : 40.f;
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units; scale > 0
-        float m = -INFINITY;  // running maximum, in log2 units
-        float2 l2 = make_float2(0.f, 0.f);
-        bool ok = true;
-        for (uint32_t i = 0; i < n; ++i)
+        uint32_t g = 0, done = 0;  // halves and items of this tile so far
+        Item it;
+        for (uint32_t k = 0; take(k, &it); ++k)
         {
-            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_S0 + 2 * x + (i & 1u)], i >> 1, abort));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t k0 = i * KH, ts = tx + KH * (i & 1u);
-            const bool masked = k0 + KH > least;  // the same in the whole warp
-            const int reach = (int)min(seen - k0, (uint32_t)KH) * (seen > k0);  // keys of this half that the row sees
-            // P against the maximum so far; where a row's maximum has risen too
-            // far, its output is rescaled and P computed again (as is the first)
-            uint32_t w[32];
-            float2 sum;
-            while (true)
+            const uint32_t n = x ? it.n1 : it.n0;
+            const bool live = tok < (x ? it.tok1 : it.tok0) && head < min(a.gs, a.group - it.hc);
+            const uint32_t token = it.p.t0 + (x ? a.tpt : 0u) + tok;
+            // keys the row sees; rows that are no query's are left unmasked
+            const uint32_t seen = live ? keys_seen(it.p, token) : 0xffffffffu;
+            const uint32_t least = __reduce_min_sync(FULL_MASK, seen);
+            float m = -INFINITY;  // the row's reference, in log2 units
+            float2 l2 = make_float2(0.f, 0.f);
+            bool ok = true;
+            for (uint32_t i = 0; i < n; ++i, ++g)
             {
-                const float base = m == -INFINITY ? 0.f : LIFT - m;  // no key yet: 2^(-inf) = 0
-                const float2 scale2 = make_float2(sl2, sl2), base2 = make_float2(base, base);
-                uint32_t u[2][32];
-                tmem_ld32_async(ts, u[0]);
-                tmem_ld32_async(ts + 32, u[1]);
-                sum = make_float2(0.f, 0.f);
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tmem_wait_ld(u[0]);
-                tmem_wait_ld(u[1]);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
+                if (!(ok = wait(B_S0 + 2 * x + (g & 1u), g >> 1))) break;
+                tc_fence_after();
+                const uint32_t k0 = i * KH, ts = tx + KH * (g & 1u);
+                const bool masked = k0 + KH > least;  // the same in the whole warp
+                const int reach = (int)min(seen - k0, (uint32_t)KH) * (seen > k0);  // keys of this half that the row sees
+                // P against the reference; where a score has risen too far over
+                // it, the output is rescaled and P computed again (as is the first)
+                uint32_t w[32];
+                float2 sum;
+                while (true)
                 {
-                    mask32(u[c], masked, reach - 32 * c);
+                    const float base = m == -INFINITY ? 0.f : LIFT - m;  // no key yet: 2^(-inf) = 0
+                    const float2 scale2 = make_float2(sl2, sl2), base2 = make_float2(base, base);
+                    uint32_t u[2][32];
+                    tmem_ld32_async(ts, u[0]);
+                    tmem_ld32_async(ts + 32, u[1]);
+                    sum = make_float2(0.f, 0.f);
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_wait_ld(u[0]);
+                    tmem_wait_ld(u[1]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
+                    for (int c = 0; c < 2; ++c)
                     {
-                        const float s0 = __uint_as_float(u[c][2 * j]), s1 = __uint_as_float(u[c][2 * j + 1]);
-                        mx[j & 3] = max3(mx[j & 3], s0, s1);
-                        const float2 e = fma2(make_float2(s0, s1), scale2, base2);
-                        const float2 q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
-                        sum = add2(sum, q);
-                        w[16 * c + j] = pack2<T>(q.x, q.y);
+                        mask32(u[c], masked, reach - 32 * c);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                        {
+                            const float s0 = __uint_as_float(u[c][2 * j]), s1 = __uint_as_float(u[c][2 * j + 1]);
+                            mx[j & 3] = max3(mx[j & 3], s0, s1);
+                            const float2 e = fma2(make_float2(s0, s1), scale2, base2);
+                            const float2 q = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                            sum = add2(sum, q);
+                            w[16 * c + j] = pack2<T>(q.x, q.y);
+                        }
+                    }
+                    const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
+                    const bool need = mt > m + RISE;
+                    if (!__any_sync(FULL_MASK, need)) break;
+                    const float mn = need ? mt : m;
+                    const float corr = need ? ex2_approx(m - mn) : 1.0f;
+                    l2.x *= corr;
+                    l2.y *= corr;
+                    m = mn;
+                    if (i > 0)
+                    {
+                        // the product of the half before must have gone into the
+                        // output (the one before it has: S was issued after it)
+                        if (!(ok = wait(B_O0 + 2 * x + ((g - 1) & 1u), (g - 1) >> 1))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32)
+                        {
+                            float v[32];
+                            uint32_t o[32];
+                            tmem_ld32(tx + Sh::O + c, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j] * corr);
+                            tmem_st32(tx + Sh::O + c, o);
+                        }
                     }
                 }
-                const float mt = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * sl2;
-                const bool need = mt > m + RISE;
-                if (!__any_sync(FULL_MASK, need)) break;
-                const float mn = need ? mt : m;
-                const float corr = need ? ex2_approx(m - mn) : 1.0f;
-                l2.x *= corr;
-                l2.y *= corr;
-                m = mn;
-                if (i > 0)
-                {
-                    // the product of half i - 1 must have gone into the output
-                    // (that of i - 2 has: S of half i was issued after it)
-                    if (!(ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_O0 + x], i - 1, abort)))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32)
-                    {
-                        float v[32];
-                        uint32_t o[32];
-                        tmem_ld32(tx + Sh::O + c, v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(v[j] * corr);
-                        tmem_st32(tx + Sh::O + c, o);
-                    }
-                }
+                if (!ok) break;
+                l2 = add2(l2, sum);
+                tmem_st32(ts, w);  // over scores that have been read
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bars[B_P0 + 2 * x + (g & 1u)]);
             }
             if (!ok) break;
-            l2 = add2(l2, sum);
-            tmem_st32(ts, w);  // over scores that have been read
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&bars[B_P0 + 2 * x + (i & 1u)]);
-        }
-        if (ok && n > 0)
-        {
-            // every product of the tile is done (a barrier of one phase: this
-            // thread has not followed the output's, and may be two behind)
-            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[B_FIN + x], 0, abort));
-            tc_fence_after();
-        }
-        if (ok)
-        {
+            // The output, 32 columns at a time through shared memory: rows lie
+            // far apart, and a store of 16 bytes of each of 32 rows costs the
+            // memory unit 32 steps, one of 64 bytes of 8 rows 8.
             const float l = l2.x + l2.y, inv = l == 0.f ? 0.f : 1.0f / l;
-            T* dst = out + (uint64_t)(p.q0 + token) * a.ldo + (uint64_t)(kvh * a.group + hc + head) * HD;
-            if (n == 0)
+            if (n > 0 && !wait(B_OD + x, done++)) break;
+            tc_fence_after();
+            const uint64_t row = (uint64_t)(it.p.q0 + token) * a.ldo + (uint64_t)(it.kvh * a.group + it.hc + head) * HD;
+            uint4* stage = staging + warp * 128;  // 32 rows of 4 x 16 bytes, chunk j of row i at j ^ (i >> 1 & 3)
+#pragma unroll
+            for (int c = 0; c < HD; c += 32)
             {
-                if (live)
-                    for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            else
-#pragma unroll
-                for (int c = 0; c < HD; c += 32)
+                float v[32];
+                if (n > 0)
                 {
-                    float v[32];
                     tmem_ld32(tx + Sh::O + c, v);
-                    if (live)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(dst + c + i) =
-                                seen ? make_uint4(pack2<T>(v[i] * inv, v[i + 1] * inv), pack2<T>(v[i + 2] * inv, v[i + 3] * inv),
-                                                  pack2<T>(v[i + 4] * inv, v[i + 5] * inv), pack2<T>(v[i + 6] * inv, v[i + 7] * inv))
-                                     : make_uint4(0u, 0u, 0u, 0u);
+                    if (c + 32 == HD)
+                    {
+                        tc_fence_before();
+                        mbar_arrive(&bars[B_OE + x]);  // the next item's products may overwrite the output
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const uint4 q = make_uint4(pack2<T>(v[8 * j] * inv, v[8 * j + 1] * inv), pack2<T>(v[8 * j + 2] * inv, v[8 * j + 3] * inv),
+                                               pack2<T>(v[8 * j + 4] * inv, v[8 * j + 5] * inv), pack2<T>(v[8 * j + 6] * inv, v[8 * j + 7] * inv));
+                    stage[4 * lane + (j ^ (lane >> 1 & 3))] = n > 0 && seen ? q : make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const int i = 8 * j + (lane >> 2);  // row of the warp; 4 lanes each
+                    const uint64_t at = __shfl_sync(FULL_MASK, row, i);
+                    const bool there = __shfl_sync(FULL_MASK, (int)live, i);
+                    const uint4 q = stage[4 * i + ((lane & 3) ^ (i >> 1 & 3))];
+                    if (there) *reinterpret_cast<uint4*>(out + at + c + 8 * (lane & 3)) = q;
+                }
+                __syncwarp();
+            }
         }
     }
     else if (warp < 10)
     {
-        // ---------------- MMA issue for tile x ----------------
+        // ---------------- S of tile x ----------------
         const int x = warp - 8;
-        const uint32_t n = x ? n1 : n0;
-        if (n > 0)
+        const uint64_t dq = Sh::KDESC | (uint64_t)(smem_u32(q_s + x * Sh::TILE) >> 4);
+        const uint64_t dk = Sh::KDESC | (uint64_t)(smem_u32(k_s) >> 4);
+        const uint32_t ts = tmem + Sh::TX * x;
+        uint32_t g = 0, tiles = 0, queries = 0;  // halves, key tiles and items so far
+        bool ok = true;
+        Item it;
+        for (uint32_t k = 0; ok && take(k, &it); ++k)
         {
-            auto wait = [&](int b, uint32_t ph) { return __all_sync(FULL_MASK, mbar_wait_or(&bars[b], ph, abort)); };
-            const uint64_t dq = Sh::KDESC | (uint64_t)(smem_u32(q_s + x * Sh::TILE) >> 4);
-            const uint64_t dk = Sh::KDESC | (uint64_t)(smem_u32(k_s) >> 4);
-            const uint64_t dv = Sh::VDESC | (uint64_t)(smem_u32(v_s) >> 4);
-            const uint32_t ts = tmem + Sh::TX * x, to = ts + Sh::O;
-            // S of half i into its buffer; the last half of a key tile frees it
-            auto scores = [&](uint32_t i) {
-                const uint32_t st = (i >> 1) % ST, buf = i & 1u;
-                const uint64_t kb = dk + ((st * Sh::TILE + buf * KH * Sh::ROW) >> 4);
-                tc_fence_after();
-#pragma unroll
-                for (int j = 0; j < Sh::BOXES; ++j)
-#pragma unroll
-                    for (int kk = 0; kk < Sh::COLS / 16; ++kk)
-                    {
-                        const uint32_t off = (j * Sh::BOX + kk * 32) >> 4;
-                        mma_f16_ss(ts + KH * buf, dq + off, kb + off, IDESC_S, j > 0 || kk > 0);
-                    }
-                commit(&bars[B_S0 + 2 * x + buf]);
-                if (buf || i + 1 == n) commit(&bars[Bx::KE + ST * x + st]);
-            };
-            bool ok = wait(B_QF, 0) && wait(Bx::KF, 0);
-            if (ok) scores(0);
-            if (ok && n > 1) scores(1);
-            for (uint32_t i = 0; ok && i < n; ++i)
+            if (it.ntiles == 0) continue;
+            const uint32_t n = uniform(x ? it.n1 : it.n0), ntiles = uniform(it.ntiles);
+            if (!(ok = wait(B_QF, queries++))) break;
+            for (uint32_t t = 0; ok && t < ntiles; ++t, ++tiles)
             {
-                const uint32_t t = i >> 1, st = t % ST, buf = i & 1u;
-                if (!buf)
-                {
-                    if (!(ok = wait(Bx::VF + st, t / ST))) break;
-                    if (t == ntiles - 1 && tail < KT && !(ok = wait(B_VR, 0))) break;
-                }
-                // O += P V of half i
-                if (!(ok = wait(B_P0 + 2 * x + buf, t))) break;
-                tc_fence_after();
+                const uint32_t st = tiles % ST;
+                if (!(ok = wait(Bx::KF + st, tiles / ST))) break;
 #pragma unroll
-                for (int kk = 0; kk < KH / 16; ++kk)
-                    mma_f16_ts(to, ts + KH * buf + 8 * kk, dv + ((st * Sh::TILE + (buf * KH + kk * 16) * Sh::ROW) >> 4),
-                               IDESC_O, i > 0 || kk > 0);
-                commit(&bars[B_O0 + x]);
-                if (buf || i + 1 == n) commit(&bars[Bx::VE + ST * x + st]);
-                if (i + 2 < n)
-                {
-                    // S of half i + 2, once P of half i, in the same buffer, has been read
-                    if (!buf && !(ok = wait(Bx::KF + (t + 1) % ST, (t + 1) / ST))) break;
-                    if (!(ok = wait(B_O0 + x, i))) break;
-                    scores(i + 2);
-                }
+                for (uint32_t half = 0; half < 2; ++half)
+                    if (2 * t + half < n)
+                    {
+                        // its buffer: P V of the half before last has read it
+                        if (g >= 2 && !(ok = wait(B_O0 + 2 * x + (g & 1u), (g >> 1) - 1))) break;
+                        const uint64_t kb = dk + ((st * Sh::TILE + half * KH * Sh::ROW) >> 4);
+                        tc_fence_after();
+#pragma unroll
+                        for (int j = 0; j < Sh::BOXES; ++j)
+#pragma unroll
+                            for (int kk = 0; kk < Sh::COLS / 16; ++kk)
+                            {
+                                const uint32_t off = (j * Sh::BOX + kk * 32) >> 4;
+                                mma_f16_ss(ts + KH * (g & 1u), dq + off, kb + off, IDESC_S, j > 0 || kk > 0);
+                            }
+                        commit(&bars[B_S0 + 2 * x + (g & 1u)]);
+                        ++g;
+                    }
+                if (!ok) break;
+                commit(&bars[Bx::KE + st]);  // a tile is given back, used or not
             }
-            // every MMA this warp issued completes before TMEM is freed
-            commit(&bars[B_FIN + x]);
-            __all_sync(FULL_MASK, mbar_wait(&bars[B_FIN + x], 0));
+            if (ok) commit(&bars[B_QE]);
         }
+        // every MMA this warp issued completes before TMEM is freed
+        commit(&bars[B_FIN + x]);
+        __all_sync(FULL_MASK, mbar_wait(&bars[B_FIN + x], 0));
     }
-    else if (warp == 10)
+    else if (warp < 12)
+    {
+        // ---------------- P V of tile x ----------------
+        const int x = warp - 10;
+        const uint64_t dv = Sh::VDESC | (uint64_t)(smem_u32(v_s) >> 4);
+        const uint32_t ts = tmem + Sh::TX * x, to = ts + Sh::O;
+        // halves, key tiles and items of this query tile so far; by stage, zeroed tiles' parity
+        uint32_t g = 0, tiles = 0, outputs = 0, ends = 0;
+        bool ok = true;
+        Item it;
+        for (uint32_t k = 0; ok && take(k, &it); ++k)
+        {
+            if (it.ntiles == 0) continue;
+            const uint32_t n = uniform(x ? it.n1 : it.n0), ntiles = uniform(it.ntiles), tail = uniform(it.tail);
+            for (uint32_t t = 0; ok && t < ntiles; ++t, ++tiles)
+            {
+                const uint32_t st = tiles % ST;
+                if (!(ok = wait(Bx::VF + st, tiles / ST))) break;
+                if (t + 1 == ntiles && tail < KT)
+                {
+                    if (!(ok = wait(Bx::VR + st, ends >> st & 1u))) break;
+                    ends ^= 1u << st;
+                }
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half)
+                    if (2 * t + half < n)
+                    {
+                        // the item's first overwrites an output that has been read
+                        if (t == 0 && half == 0 && outputs > 0 && !(ok = wait(B_OE + x, outputs - 1))) break;
+                        if (!(ok = wait(B_P0 + 2 * x + (g & 1u), g >> 1))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < KH / 16; ++kk)
+                            mma_f16_ts(to, ts + KH * (g & 1u) + 8 * kk,
+                                       dv + ((st * Sh::TILE + (half * KH + kk * 16) * Sh::ROW) >> 4), IDESC_O,
+                                       t > 0 || half > 0 || kk > 0);
+                        commit(&bars[B_O0 + 2 * x + (g & 1u)]);
+                        if (2 * t + half + 1 == n) commit(&bars[B_OD + x]);
+                        ++g;
+                    }
+                if (!ok) break;
+                commit(&bars[Bx::VE + st]);
+            }
+            outputs += n > 0;
+        }
+        commit(&bars[B_FIN + 2 + x]);
+        __all_sync(FULL_MASK, mbar_wait(&bars[B_FIN + 2 + x], 0));
+    }
+    else if (warp == 12)
     {
         // ---------------- TMA copies ----------------
-        uint32_t last = 0;  // copies issued
-        if (lane == 0 && ntiles > 0)
+        uint32_t tiles = 0, queries = 0;  // so far
+        uint32_t kcopies = 0, vcopies = 0, qcopies = 0;
+        Item it;
+        for (uint32_t k = 0; take(k, &it); ++k)
         {
-            const uint32_t nq = nt1 ? 2u : 1u;
-            mbar_arrive_expect_tx(&bars[B_QF], nq * Sh::BOXES * a.gs * a.tpt * Sh::ROW);
-            for (uint32_t x = 0; x < nq; ++x)
-                for (int j = 0; j < Sh::BOXES; ++j)
-                    tma_load_3d(q_s + x * Sh::TILE + j * Sh::BOX, &map_q, Sh::COLS * j, (int)(kvh * a.group + hc),
-                                (int)(p.q0 + p.t0 + x * a.tpt), &bars[B_QF]);
-            uint32_t issued = 0;  // copies: K(t) is 2 t, V(t) is 2 t + 1
-            for (uint32_t t = 0; t < ntiles; ++t)
+            if (it.ntiles == 0) continue;
+            if (queries > 0 && !wait(B_QE, queries - 1)) break;
+            if (lane == 0)
             {
-                const uint32_t st = t % ST, ph = t / ST;
+                const uint32_t nq = it.tok1 ? 2u : 1u;
+                mbar_arrive_expect_tx(&bars[B_QF], nq * Sh::BOXES * a.gs * a.tpt * Sh::ROW);
+                for (uint32_t x = 0; x < nq; ++x)
+                    for (int j = 0; j < Sh::BOXES; ++j)
+                        tma_load_3d(q_s + x * Sh::TILE + j * Sh::BOX, &map_q, Sh::COLS * j, (int)(it.kvh * a.group + it.hc),
+                                    (int)(it.p.q0 + it.p.t0 + x * a.tpt), &bars[B_QF]);
+            }
+            ++qcopies;
+            bool ok = true;
+            for (uint32_t t = 0; t < it.ntiles; ++t)
+            {
+                const uint32_t tile = tiles + t, st = tile % ST, ph = tile / ST;
                 // into stage st once both query tiles' products have read what it held
-                auto freed = [&](int e) {
-                    return t < (uint32_t)ST || ((t - ST >= nt0 || mbar_wait_or(&bars[e + st], ph - 1, abort)) &&
-                                                (t - ST >= nt1 || mbar_wait_or(&bars[e + ST + st], ph - 1, abort)));
-                };
-                if (!freed(Bx::KE)) break;
-                mbar_arrive_expect_tx(&bars[Bx::KF + st], Sh::TILE);
-                for (int j = 0; j < Sh::BOXES; ++j)
-                    tma_load_2d(k_s + st * Sh::TILE + j * Sh::BOX, &map_k, (int)(kvh * HD) + Sh::COLS * j,
-                                (int)(p.k0 + t * KT), &bars[Bx::KF + st]);
-                issued = 2 * t + 1;
-                if (!freed(Bx::VE)) break;
-                mbar_arrive_expect_tx(&bars[Bx::VF + st], Sh::TILE);
-                for (int j = 0; j < Sh::BOXES; ++j)
-                    tma_load_2d(v_s + st * Sh::TILE + j * Sh::BOX, &map_v, (int)(kvh * HD) + Sh::COLS * j,
-                                (int)(p.k0 + t * KT), &bars[Bx::VF + st]);
-                issued = 2 * t + 2;
-            }
-            last = issued;
-        }
-        // Rows past the sequence's end in its last value tile.  The copy loop
-        // has seen every earlier phase of the stage's barrier complete.
-        __syncwarp();
-        last = __shfl_sync(FULL_MASK, last, 0);
-        if (tail < KT && ntiles > 0 && last == 2 * ntiles)
-        {
-            const uint32_t st = (ntiles - 1) % ST;
-            if (mbar_wait_or(&bars[Bx::VF + st], (ntiles - 1) / ST, abort))
-            {
-                for (int j = 0; j < Sh::BOXES; ++j)
+                if (ph > 0 && !(ok = wait(Bx::KE + st, ph - 1))) break;
+                if (lane == 0)
                 {
-                    uint4* box = reinterpret_cast<uint4*>(v_s + st * Sh::TILE + j * Sh::BOX);
-                    for (uint32_t i = tail * (Sh::ROW / 16) + lane; i < Sh::BOX / 16; i += 32)
-                        box[i] = make_uint4(0u, 0u, 0u, 0u);
+                    mbar_arrive_expect_tx(&bars[Bx::KF + st], Sh::TILE);
+                    for (int j = 0; j < Sh::BOXES; ++j)
+                        tma_load_2d(k_s + st * Sh::TILE + j * Sh::BOX, &map_k, (int)(it.kvh * HD) + Sh::COLS * j,
+                                    (int)(it.p.k0 + t * KT), &bars[Bx::KF + st]);
                 }
-                fence_async_smem();
-                mbar_arrive(&bars[B_VR]);
+                ++kcopies;
+                if (ph > 0 && !(ok = wait(Bx::VE + st, ph - 1))) break;
+                if (lane == 0)
+                {
+                    mbar_arrive_expect_tx(&bars[Bx::VF + st], Sh::TILE);
+                    for (int j = 0; j < Sh::BOXES; ++j)
+                        tma_load_2d(v_s + st * Sh::TILE + j * Sh::BOX, &map_v, (int)(it.kvh * HD) + Sh::COLS * j,
+                                    (int)(it.p.k0 + t * KT), &bars[Bx::VF + st]);
+                }
+                ++vcopies;
+                if (t + 1 == it.ntiles && it.tail < KT)
+                {
+                    // rows past the sequence's end
+                    if (!(ok = wait(Bx::VF + st, ph))) break;
+                    for (int j = 0; j < Sh::BOXES; ++j)
+                    {
+                        uint4* box = reinterpret_cast<uint4*>(v_s + st * Sh::TILE + j * Sh::BOX);
+                        for (uint32_t i = it.tail * (Sh::ROW / 16) + lane; i < Sh::BOX / 16; i += 32)
+                            box[i] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_async_smem();
+                    mbar_arrive(&bars[Bx::VR + st]);
+                }
             }
+            if (!ok) break;
+            tiles += it.ntiles;
+            ++queries;
         }
-        if (lane == 0 && ntiles > 0)
+        // the copies this warp started land before the CTA exits (bounded)
+        if (qcopies > 0) mbar_wait(&bars[B_QF], (qcopies - 1) & 1u);
+        for (uint32_t i = kcopies > ST ? kcopies - ST : 0; i < kcopies; ++i) mbar_wait(&bars[Bx::KF + i % ST], (i / ST) & 1u);
+        for (uint32_t i = vcopies > ST ? vcopies - ST : 0; i < vcopies; ++i) mbar_wait(&bars[Bx::VF + i % ST], (i / ST) & 1u);
+    }
+    else if (warp == 13)
+    {
+        // ---------------- the next item ----------------
+        const uint32_t ny = a.kv_heads * a.nchunk;
+        PackedArgs pair = a;  // an item has two tiles of a.tpt tokens
+        pair.tpt = 2 * a.tpt;
+        uint32_t asked = 0;
+        bool more = true;
+        uint32_t block = blockIdx.x;
+        for (uint32_t k = 0; more;)
         {
-            // the copies this thread started land before the CTA exits (bounded)
-            mbar_wait(&bars[B_QF], 0);
-            for (uint32_t n = last > 2 * ST ? last - 2 * ST : 0; n < last; ++n)
+            Item it;
+            it.p = packed_tile_warp(pair, block / ny);
+            // ask for the next block while this one is worked out
+            if (lane == 0)
             {
-                const uint32_t t = n >> 1;
-                mbar_wait(&bars[(n & 1u ? Bx::VF : Bx::KF) + t % ST], (t / ST) & 1u);
+                mbar_arrive_expect_tx(&bars[B_CL], 16);
+                cuda::ptx::clusterlaunchcontrol_try_cancel(answer, &bars[B_CL]);
+            }
+            if (it.p.live)
+            {
+                const uint32_t y = block % ny;
+                it.kvh = y / a.nchunk;
+                it.hc = (y % a.nchunk) * a.gs;
+                const uint32_t tokens = min(pair.tpt, it.p.lq - it.p.t0);
+                it.tok0 = min(a.tpt, tokens);
+                it.tok1 = tokens - it.tok0;
+                it.n0 = (keys_seen(it.p, it.p.t0 + it.tok0 - 1) + KH - 1) / KH;
+                it.n1 = it.tok1 ? (keys_seen(it.p, it.p.t0 + tokens - 1) + KH - 1) / KH : 0u;
+                it.ntiles = (max(it.n0, it.n1) + 1) / 2;
+                it.tail = it.ntiles ? min((uint32_t)KT, it.p.lk - (it.ntiles - 1) * KT) : (uint32_t)KT;
+                if (k >= 2 && !wait(B_TE + (k & 1u), (k >> 1) - 1)) break;
+                if (lane == 0)
+                {
+                    items[k & 1u] = it;
+                    mbar_arrive(&bars[B_TF + (k & 1u)]);
+                }
+                ++k;
+            }
+            if (!wait(B_CL, asked++)) break;
+            const uint4 got = *answer;
+            more = cuda::ptx::clusterlaunchcontrol_query_cancel_is_canceled(got);
+            if (more) block = (uint32_t)cuda::ptx::clusterlaunchcontrol_query_cancel_get_first_ctaid_x<int>(got);
+            __syncwarp();
+            fence_async_smem();  // the answer has been read before the next one is written
+            if (!more)
+            {
+                if (k >= 2 && !wait(B_TE + (k & 1u), (k >> 1) - 1)) break;
+                if (lane == 0)
+                {
+                    items[k & 1u].p.live = 0;
+                    mbar_arrive(&bars[B_TF + (k & 1u)]);
+                }
             }
         }
     }
