@@ -143,5 +143,7 @@ inline uint64_t packed_tiles_bound(const PackedArgs& a) { return (uint64_t)a.q_r
 
 int launch_packed_attention_tc(void* out, const void* q, const void* k, const void* v, int type, uint32_t head_dim,
                                const PackedArgs& a, cudaStream_t st);
+int launch_packed_attention_tf32(float* out, const float* q, const float* k, const float* v, uint32_t hd,
+                                 const PackedArgs& p, bool split3, cudaStream_t st);
 
 }  // namespace fml

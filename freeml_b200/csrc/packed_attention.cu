@@ -216,6 +216,13 @@ extern "C" int fml_attention_packed(void* out, const void* q, const void* k, con
         const int rc = launch_packed_attention_tc(out, q, k, v, type, head_dim, a, st);
         if (rc != FML_ERR_UNSUPPORTED) return rc;
     }
+    else if (mode != FML_MATH_FP32)
+    {
+        const int rc = launch_packed_attention_tf32(static_cast<float*>(out), static_cast<const float*>(q),
+                                                    static_cast<const float*>(k), static_cast<const float*>(v), head_dim, a,
+                                                    mode == FML_MATH_TF32X3, st);
+        if (rc != FML_ERR_UNSUPPORTED) return rc;
+    }
     auto go = [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if (head_dim == 32) return launch_simt<T, 32>(out, q, k, v, a, st);

@@ -157,15 +157,6 @@ __device__ __forceinline__ void commit(uint64_t* bar)
         : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(tc::smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
-        : "memory");
-}
-
 // A value that is the same in the whole warp, as the compiler cannot see: an
 // operand of it then needs no loop over the lanes' values.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(FULL_MASK, x, 0); }

@@ -23,9 +23,14 @@
 // start as soon as the MMAs that read the current ones have completed.
 // Every mbarrier wait is bounded (expiries are counted in the device error
 // count; the CTA then stops issuing work and still frees its TMEM).
+//
+// PACKED: the same over packed prompts with grouped heads (packed.cuh): the
+// CTA's rows are (token, query head) pairs of one key/value head, each with the
+// number of keys that it sees.
 #include <cmath>
 #include <cstdlib>
 
+#include "packed.cuh"
 #include "tcgen05.cuh"
 
 namespace fml {
@@ -57,9 +62,10 @@ struct PfShape
     static constexpr uint32_t TCOLS = OCOL + HD <= 128 ? 128 : 256;
 };
 
+template <bool ROUND>
 __device__ __forceinline__ void lo_inplace(float4* dst, const float4* src, uint32_t n4, int tid)
 {
-    for (uint32_t i = tid; i < n4; i += 128) dst[i] = tc::tf32_lo4(src[i]);
+    for (uint32_t i = tid; i < n4; i += 128) dst[i] = tc::tf32_lo4_as<ROUND>(src[i]);
 }
 
 __device__ __forceinline__ uint64_t desc_mn(const void* tile)
@@ -72,11 +78,11 @@ __device__ __forceinline__ uint64_t desc_mn(const void* tile)
 
 }  // namespace
 
-template <int HD, bool SPLIT3>
+template <int HD, bool SPLIT3, bool PACKED>
 __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v,
-                                                                      PfArgs a)
+                                                                      PfArgs a, PackedArgs pk)
 {
     using namespace tc;
     using Sh = PfShape<HD>;
@@ -100,12 +106,29 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     enum { BQ = 0, BKEY = 1, BVAL = 2, BS = 3, BO = 4 };
 
     const int tid = threadIdx.x, warp = tid >> 5;
-    const uint32_t q0 = blockIdx.x * QB, h = blockIdx.y, b = blockIdx.z;
+    const uint32_t q0 = PACKED ? 0u : blockIdx.x * QB, h = blockIdx.y, b = blockIdx.z;
     const uint32_t P = a.P;
-    const uint32_t nkeys = min(q0 + (uint32_t)QB, P);         // keys this CTA's rows can see
-    const uint32_t ntiles = (nkeys + KT - 1) / KT;
-    const int kv_row0 = (int)((b * a.H + h) * a.C);           // this (sequence, head)'s first cache row
+    uint32_t nkeys = min(q0 + (uint32_t)QB, P);               // keys this CTA's rows can see
+    int kv_row0 = (int)((b * a.H + h) * a.C), kv_col0 = 0;    // this (sequence, head)'s first cache row
     const uint32_t q = q0 + tid;                              // this thread's query row
+    uint32_t sees = 0, q_row = b * P + q, q_head = h;         // PACKED: keys it sees; its place in q and out
+    bool live = q < P;
+    PackedTile pt{};
+    if constexpr (PACKED)
+    {
+        pt = packed_tile<128>(pk, blockIdx.x);
+        if (!pt.live) return;
+        const uint32_t kvh = h / pk.nchunk, hc = (h % pk.nchunk) * pk.gs, tok = tid / pk.gs, head = tid % pk.gs;
+        const uint32_t tokens = min(pk.tpt, pt.lq - pt.t0);
+        live = tok < tokens && head < min(pk.gs, pk.group - hc);
+        nkeys = keys_seen(pt, pt.t0 + tokens - 1);
+        sees = live ? keys_seen(pt, pt.t0 + tok) : 0u;
+        kv_row0 = (int)pt.k0;
+        kv_col0 = (int)(kvh * HD);
+        q_row = pt.q0 + pt.t0 + tok;
+        q_head = kvh * pk.group + hc + head;
+    }
+    const uint32_t ntiles = (nkeys + KT - 1) / KT;
     // thread 0's count of the phases it started / saw complete on each barrier
     // (the drain after an expired wait)
     uint32_t issued[5] = {0, 0, 0, 0, 0}, seen[5] = {0, 0, 0, 0, 0};
@@ -132,15 +155,15 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     auto issue_k = [&](uint32_t t) {
         mbar_arrive_expect_tx(&bars[BKEY], Sh::KBYTES);
         for (int j = 0; j < HD / 32; ++j)
-            tma_load_2d(k_s + j * (KT * 128), &map_k, 32 * j, kv_row0 + (int)(t * KT), &bars[BKEY]);
+            tma_load_2d(k_s + j * (KT * 128), &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * KT), &bars[BKEY]);
         ++issued[BKEY];
     };
     auto issue_v = [&](uint32_t t) {
         mbar_arrive_expect_tx(&bars[BVAL], Sh::VBYTES);
         for (int kb = 0; kb < KT / 32; ++kb)
             for (int j = 0; j < HD / 32; ++j)
-                tma_load_2d(v_s + (kb * (HD / 32) + j) * 4096, &map_v, 32 * j, kv_row0 + (int)(t * KT) + 32 * kb,
-                            &bars[BVAL]);
+                tma_load_2d(v_s + (kb * (HD / 32) + j) * 4096, &map_v, kv_col0 + 32 * j,
+                            kv_row0 + (int)(t * KT) + 32 * kb, &bars[BVAL]);
         ++issued[BVAL];
     };
     // bounded wait on phase `ph` of barrier i, the same answer in the whole warp
@@ -151,18 +174,24 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     };
     if (tid == 0)
     {
-        mbar_arrive_expect_tx(&bars[BQ], Sh::QBYTES);
+        mbar_arrive_expect_tx(&bars[BQ], PACKED ? (HD / 32) * pk.gs * pk.tpt * 128 : Sh::QBYTES);
         for (int j = 0; j < HD / 32; ++j)
-            tma_load_2d(q_s + j * (QB * 128), &map_q, (int)(h * HD) + 32 * j, (int)(b * P + q0), &bars[BQ]);
+            if constexpr (PACKED)  // thread 0's row is the tile's first
+                tma_load_3d(q_s + j * (QB * 128), &map_q, 32 * j, (int)q_head, (int)q_row, &bars[BQ]);
+            else
+                tma_load_2d(q_s + j * (QB * 128), &map_q, (int)(h * HD) + 32 * j, (int)(b * P + q0), &bars[BQ]);
         issued[BQ] = 1;
-        issue_k(0);
-        issue_v(0);
+        if (!PACKED || ntiles > 0)
+        {
+            issue_k(0);
+            issue_v(0);
+        }
     }
 
     bool ok = wait(BQ, 0);
     if constexpr (SPLIT3)
         if (ok)
-            lo_inplace(reinterpret_cast<float4*>(qlo_s), reinterpret_cast<const float4*>(q_s), Sh::QBYTES / 16, tid);
+            lo_inplace<PACKED>(reinterpret_cast<float4*>(qlo_s), reinterpret_cast<const float4*>(q_s), Sh::QBYTES / 16, tid);
 
     float o[HD];
 #pragma unroll
@@ -176,7 +205,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         if (ok) ok = wait(BKEY, t);
         if constexpr (SPLIT3)
             if (ok)
-                lo_inplace(reinterpret_cast<float4*>(klo_s), reinterpret_cast<const float4*>(k_s), Sh::KBYTES / 16,
+                lo_inplace<PACKED>(reinterpret_cast<float4*>(klo_s), reinterpret_cast<const float4*>(k_s), Sh::KBYTES / 16,
                            tid);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -229,8 +258,8 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         for (int i = 0; i < KT; ++i)
         {
             const uint32_t key = k0 + i;
-            const bool live = key <= q && key < P;
-            sv[i] = live ? sv[i] * a.scale : -INFINITY;  // a select: masked slots may hold anything
+            const bool in = PACKED ? key < sees : key <= q && key < P;
+            sv[i] = in ? sv[i] * a.scale : -INFINITY;  // a select: masked slots may hold anything
             mx = fmaxf(mx, sv[i]);
         }
         const float corr = m == -INFINITY ? 0.f : expf(m - mx);
@@ -254,7 +283,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
                                               sv[kb * 32 + 4 * c + 3]);
                 const uint32_t off = kb * (QB * 128) + tid * 128 + ((c ^ (tid & 7)) * 16);
                 *reinterpret_cast<float4*>(p_s + off) = pv;
-                if constexpr (SPLIT3) *reinterpret_cast<float4*>(plo_s + off) = tf32_lo4(pv);
+                if constexpr (SPLIT3) *reinterpret_cast<float4*>(plo_s + off) = tf32_lo4_as<PACKED>(pv);
             }
 
         // ---- O_tile = P V ----
@@ -279,7 +308,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
                         if constexpr (SPLIT3) vlo4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
                     else if constexpr (SPLIT3)
-                        vlo4[i] = tf32_lo4(v4[i]);
+                        vlo4[i] = tf32_lo4_as<PACKED>(v4[i]);
                 }
             }
         }
@@ -324,10 +353,11 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     }
     ok = __syncthreads_and(ok) != 0;
 
-    if (ok && q < P)
+    if (ok && live)
     {
-        const float inv = 1.0f / l;  // l >= 1: the row's largest score contributes exp(0)
-        float* dst = a.out + (uint64_t)(b * P + q) * a.ldo + h * HD;
+        // l >= 1: the row's largest score contributes exp(0); a packed row may see no key
+        const float inv = PACKED && sees == 0 ? 0.f : 1.0f / l;
+        float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
 #pragma unroll
         for (int e = 0; e < HD; e += 4)
             *reinterpret_cast<float4*>(dst + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
@@ -409,11 +439,11 @@ constexpr uint32_t PP_TX = 256, PP_PLO = 64, PP_O = 128, PP_QLO = 192;
 
 }  // namespace
 
-template <bool SPLIT3>
+template <bool SPLIT3, bool PACKED>
 __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                              const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
-                                                                             PfArgs a)
+                                                                             PfArgs a, PackedArgs pk)
 {
     using namespace tc;
     constexpr uint32_t IDESC_S = idesc_tf32(128, PP_KT);
@@ -434,13 +464,33 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     const uint32_t qblk = gridDim.x - 1 - blockIdx.x;
     const uint32_t q0 = qblk * 256, h = blockIdx.y, b = blockIdx.z;
     const uint32_t P = a.P;
-    const bool has_b = q0 + 128 < P;
-    // key tiles of tile A / B and the keys any row of the CTA sees
-    const uint32_t nt0 = (min(q0 + 128u, P) + PP_KT - 1) / PP_KT;
-    const uint32_t nt1 = has_b ? (min(q0 + 256u, P) + PP_KT - 1) / PP_KT : 0u;
+    bool has_b = q0 + 128 < P;
+    // the keys that tile A's rows see, and any row of the CTA
+    uint32_t nkeys0 = min(q0 + 128u, P), nkeys = min(q0 + 256u, P);
+    int kv_row0 = (int)((b * a.H + h) * a.C), kv_col0 = 0;
+    PackedTile pt{};
+    uint32_t kvh = 0, hc = 0, tok0 = 0, tok1 = 0;  // PACKED: heads, tokens of tile A / B
+    if constexpr (PACKED)
+    {
+        PackedArgs pair = pk;  // a CTA has two tiles of pk.tpt tokens
+        pair.tpt = 2 * pk.tpt;
+        pt = packed_tile<PP_THREADS>(pair, blockIdx.x);
+        if (!pt.live) return;
+        kvh = h / pk.nchunk;
+        hc = (h % pk.nchunk) * pk.gs;
+        const uint32_t tokens = min(pair.tpt, pt.lq - pt.t0);
+        tok0 = min(pk.tpt, tokens);
+        tok1 = tokens - tok0;
+        has_b = tok1 > 0;
+        nkeys0 = keys_seen(pt, pt.t0 + tok0 - 1);
+        nkeys = keys_seen(pt, pt.t0 + tokens - 1);
+        kv_row0 = (int)pt.k0;
+        kv_col0 = (int)(kvh * PP_HD);
+    }
+    // key tiles of tile A / B
+    const uint32_t nt0 = (nkeys0 + PP_KT - 1) / PP_KT;
+    const uint32_t nt1 = has_b ? (nkeys + PP_KT - 1) / PP_KT : 0u;
     const uint32_t ntiles = has_b ? nt1 : nt0;
-    const uint32_t nkeys = min(q0 + 256u, P);
-    const int kv_row0 = (int)((b * a.H + h) * a.C);
 
     if (tid == 0)
     {
@@ -474,6 +524,18 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         const uint32_t nt = x ? nt1 : nt0;
         const int r = 32 * (warp & 3) + lane;                 // row within the tile
         const uint32_t row = q0 + 128u * x + (uint32_t)r;     // this thread's query row
+        uint32_t seen = 0, least = 0, q_row = b * P + row, q_head = h;  // PACKED: keys it sees, the warp's least
+        bool live = row < P;
+        if constexpr (PACKED)
+        {
+            const uint32_t tok = (uint32_t)r / pk.gs, head = (uint32_t)r % pk.gs;
+            live = tok < (x ? tok1 : tok0) && head < min(pk.gs, pk.group - hc);
+            const uint32_t token = pt.t0 + (x ? pk.tpt : 0u) + tok;
+            seen = live ? keys_seen(pt, token) : 0xffffffffu;  // rows that are no query's are left unmasked
+            least = __reduce_min_sync(FULL_MASK, seen);
+            q_row = pt.q0 + token;
+            q_head = kvh * pk.group + hc + head;
+        }
         const uint32_t tx = tmem + PP_TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
         float m = -INFINITY, l = 0.f;
@@ -491,7 +553,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 for (int c = 0; c < 8; ++c)
                 {
                     const float4 v = *reinterpret_cast<const float4*>(qrow + j * (128 * 128) + ((c ^ (r & 7)) * 16));
-                    const float4 lo = tf32_lo4(v);
+                    const float4 lo = tf32_lo4_as<PACKED>(v);
                     u[4 * c] = __float_as_uint(lo.x);
                     u[4 * c + 1] = __float_as_uint(lo.y);
                     u[4 * c + 2] = __float_as_uint(lo.z);
@@ -535,7 +597,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             // row or past the prompt (a warp-uniform test)
             const uint32_t row0 = row - lane;
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (k0 + PP_KT - 1 <= row0 && k0 + PP_KT <= P)
+            if (PACKED ? k0 + PP_KT <= least : k0 + PP_KT - 1 <= row0 && k0 + PP_KT <= P)
             {
 #pragma unroll
                 for (int i = 0; i < PP_KT; ++i)
@@ -550,7 +612,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 for (int i = 0; i < PP_KT; ++i)
                 {
                     const uint32_t key = k0 + i;
-                    s[i] = (key <= row && key < P) ? s[i] * sl2 : -INFINITY;  // a select: masked slots may hold NaN
+                    const bool in = PACKED ? key < seen : key <= row && key < P;
+                    s[i] = in ? s[i] * sl2 : -INFINITY;  // a select: masked slots may hold NaN
                     mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
                 }
             }
@@ -578,6 +641,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 }
             }
             float ls[4] = {0.f, 0.f, 0.f, 0.f};
+            const float base = PACKED && m == -INFINITY ? 0.f : m;  // a packed row may see no key
 #pragma unroll
             for (int c = 0; c < PP_KT; c += 32)
             {
@@ -585,7 +649,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                 {
-                    const float p = ex2_approx(s[c + i] - m);  // 0 for masked keys
+                    const float p = ex2_approx(s[c + i] - base);  // 0 for masked keys
                     ls[i & 3] += p;
                     s[c + i] = p;
                     u[i] = __float_as_uint(p);
@@ -594,7 +658,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 if constexpr (SPLIT3)
                 {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(s[c + i] - tf32_hi(s[c + i]));
+                    for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(tf32_lo<PACKED>(s[c + i]));
                     tmem_st32(tx + PP_PLO + c, u);
                 }
             }
@@ -609,20 +673,25 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             if (ok)
             {
                 tc_fence_after();
-                const float inv = 1.0f / l;
-                float* dst = a.out + (uint64_t)(b * P + row) * a.ldo + h * PP_HD;
+                const float inv = PACKED && seen == 0 ? 0.f : 1.0f / l;
+                float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * PP_HD;
 #pragma unroll
                 for (int c = 0; c < PP_HD; c += 32)
                 {
                     float v[32];
                     tmem_ld32(tx + PP_O + c, v);
-                    if (row < P)
+                    if (live)
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *reinterpret_cast<float4*>(dst + c + i) =
                                 make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
                 }
             }
+        }
+        if (PACKED && ok && nt == 0 && live)
+        {
+            float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * PP_HD;
+            for (int i = 0; i < PP_HD; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
     else if (warp == 8)
@@ -646,7 +715,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
 #pragma unroll
                     for (int n = 0; n < 16; ++n) v[n] = box[ct + 32 * n];
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) box[512 + ct + 32 * n] = tf32_lo4(v[n]);
+                    for (int n = 0; n < 16; ++n) box[512 + ct + 32 * n] = tf32_lo4_as<PACKED>(v[n]);
                 }
             }
             fence_async_smem();
@@ -670,7 +739,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
 #pragma unroll
                             for (int n = 0; n < 16; ++n) v[n] = blk[ct + 32 * n];
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) blk[512 + ct + 32 * n] = tf32_lo4(v[n]);
+                            for (int n = 0; n < 16; ++n) blk[512 + ct + 32 * n] = tf32_lo4_as<PACKED>(v[n]);
                         }
                     }
                     else
@@ -684,7 +753,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                                 if constexpr (SPLIT3) blk[512 + i] = make_float4(0.f, 0.f, 0.f, 0.f);
                             }
                             else if constexpr (SPLIT3)
-                                blk[512 + i] = tf32_lo4(blk[i]);
+                                blk[512 + i] = tf32_lo4_as<PACKED>(blk[i]);
                         }
                     }
                 }
@@ -765,11 +834,15 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         if (lane == 0)
         {
             const int nq = has_b ? 2 : 1;
-            mbar_arrive_expect_tx(&bars[PB_QF], nq * PP_QTILE);
+            mbar_arrive_expect_tx(&bars[PB_QF], PACKED ? nq * (PP_HD / 32) * pk.gs * pk.tpt * 128 : nq * PP_QTILE);
             for (int x = 0; x < nq; ++x)
                 for (int j = 0; j < PP_HD / 32; ++j)
-                    tma_load_2d(q_s + x * PP_QTILE + j * (128 * 128), &map_q, (int)(h * PP_HD) + 32 * j,
-                                (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
+                    if constexpr (PACKED)
+                        tma_load_3d(q_s + x * PP_QTILE + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
+                                    (int)(pt.q0 + pt.t0 + x * pk.tpt), &bars[PB_QF]);
+                    else
+                        tma_load_2d(q_s + x * PP_QTILE + j * (128 * 128), &map_q, (int)(h * PP_HD) + 32 * j,
+                                    (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
             uint32_t issued = 0;
             for (uint32_t t = 0; t < ntiles; ++t)
             {
@@ -779,7 +852,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 if (t >= 2 && t - 2 < nt1 && !mbar_wait_or(&bars[PB_KE + 2 + bf], (t >> 1) - 1, abort)) break;
                 mbar_arrive_expect_tx(&bars[PB_KF + bf], PP_KVT);
                 for (int j = 0; j < PP_HD / 32; ++j)
-                    tma_load_2d(k_op + bf * PP_KVOP + j * PP_KBOX, &map_k, 32 * j, kv_row0 + (int)(t * PP_KT),
+                    tma_load_2d(k_op + bf * PP_KVOP + j * PP_KBOX, &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * PP_KT),
                                 &bars[PB_KF + bf]);
                 // V(t) once O_A(t-2) and O_B(t-2) have
                 if ((t >= 2 && t - 2 < nt0 && !mbar_wait_or(&bars[PB_VE + bf], (t >> 1) - 1, abort)) ||
@@ -791,7 +864,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 mbar_arrive_expect_tx(&bars[PB_VF + bf], PP_KVT);
                 for (int kb = 0; kb < PP_KT / 32; ++kb)
                     for (int j = 0; j < PP_HD / 32; ++j)
-                        tma_load_2d(v_op + bf * PP_KVOP + kb * PP_VBLK + j * 4096, &map_v, 32 * j,
+                        tma_load_2d(v_op + bf * PP_KVOP + kb * PP_VBLK + j * 4096, &map_v, kv_col0 + 32 * j,
                                     kv_row0 + (int)(t * PP_KT) + 32 * kb, &bars[PB_VF + bf]);
                 issued = 2 * t + 2;
             }
@@ -824,7 +897,7 @@ int launch_tc_hd(const float* q, uint32_t ldq, const float* kc, const float* vc,
                  uint32_t B, uint32_t H, uint32_t P, float scale, cudaStream_t st)
 {
     using Sh = PfShape<HD>;
-    auto kern = prefill_attention_tc_kernel<HD, SPLIT3>;
+    auto kern = prefill_attention_tc_kernel<HD, SPLIT3, false>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Sh::SMEM, attr_devices));
     CUtensorMap mq, mk, mv;
@@ -836,7 +909,7 @@ int launch_tc_hd(const float* q, uint32_t ldq, const float* kc, const float* vc,
     FML_RC(tc::make_map(&mv, vc, (int)rows, HD, HD, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     PfArgs a{out, ldo, B, H, P, C, scale};
     dim3 grid((P + QB - 1) / QB, H, B);
-    kern<<<grid, 128, Sh::SMEM, st>>>(mq, mk, mv, a);
+    kern<<<grid, 128, Sh::SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
@@ -845,7 +918,7 @@ template <bool SPLIT3>
 int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, uint32_t C, float* out, uint32_t ldo,
               uint32_t B, uint32_t H, uint32_t P, float scale, cudaStream_t st)
 {
-    auto kern = prefill_attention_pp_kernel<SPLIT3>;
+    auto kern = prefill_attention_pp_kernel<SPLIT3, false>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)PP_SMEM, attr_devices));
     CUtensorMap mq, mk, mv;
@@ -857,12 +930,68 @@ int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, ui
     FML_RC(tc::make_map(&mv, vc, (int)rows, PP_HD, PP_HD, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     PfArgs a{out, ldo, B, H, P, C, scale};
     dim3 grid((P + 255) / 256, H, B);
-    kern<<<grid, PP_THREADS, PP_SMEM, st>>>(mq, mk, mv, a);
+    kern<<<grid, PP_THREADS, PP_SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
+    FML_LAUNCH_CHECK();
+    return FML_OK;
+}
+
+// Packed prompts: two tiles a CTA at head dim 64, else one.
+template <int HD, bool SPLIT3>
+int launch_packed(float* out, const float* q, const float* k, const float* v, PackedArgs p, cudaStream_t st)
+{
+    constexpr bool PP = HD == PP_HD;
+    constexpr uint32_t SMEM = PP ? PP_SMEM : PfShape<HD>::SMEM;
+    constexpr int KT = PP ? PP_KT : PfShape<HD>::KT;
+    p.gs = p.group < 128u ? p.group : 128u;
+    p.nchunk = (p.group + p.gs - 1) / p.gs;
+    p.tpt = 128u / p.gs;
+    PackedArgs pair = p;
+    if (PP) pair.tpt = 2 * p.tpt;
+    const uint64_t tiles = packed_tiles_bound(pair), y = (uint64_t)p.kv_heads * p.nchunk;
+    FML_REQUIRE(tiles < (1ull << 31) && y <= 65535u, "fml_attention_packed: %u rows, %u heads", p.q_rows, p.heads);
+    CUtensorMap mq, mk, mv;
+    FML_RC(tc::make_map_heads(&mq, q, HD, p.heads, p.q_rows, p.ldq, p.gs, p.tpt));
+    FML_RC(tc::make_map(&mk, k, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldk, KT));
+    FML_RC(tc::make_map(&mv, v, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldv, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
+    const PfArgs a{out, p.ldo, 0, 0, 0, 0, p.scale};
+    const dim3 grid((unsigned)tiles, (unsigned)y);
+    static uint64_t attr_devices = 0;
+    if constexpr (PP)
+    {
+        auto kern = prefill_attention_pp_kernel<SPLIT3, true>;
+        FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
+        kern<<<grid, PP_THREADS, SMEM, st>>>(mq, mk, mv, a, p);
+    }
+    else
+    {
+        auto kern = prefill_attention_tc_kernel<HD, SPLIT3, true>;
+        FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
+        kern<<<grid, 128, SMEM, st>>>(mq, mk, mv, a, p);
+    }
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
 
 }  // namespace
+
+// The packed prompt attention on fp32 inputs; FML_ERR_UNSUPPORTED (no error
+// recorded) for bases or strides that TMA does not take, or no key row at all.
+int launch_packed_attention_tf32(float* out, const float* q, const float* k, const float* v, uint32_t hd,
+                                 const PackedArgs& p, bool split3, cudaStream_t st)
+{
+    if (p.k_rows == 0 || !aligned16(out) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
+        (p.ldo | p.ldq | p.ldk | p.ldv) % 4 || p.ldk > (1u << 30) || p.ldv > (1u << 30))
+        return FML_ERR_UNSUPPORTED;
+    if (split3)
+    {
+        if (hd == 32) return launch_packed<32, true>(out, q, k, v, p, st);
+        if (hd == 64) return launch_packed<64, true>(out, q, k, v, p, st);
+        return launch_packed<128, true>(out, q, k, v, p, st);
+    }
+    if (hd == 32) return launch_packed<32, false>(out, q, k, v, p, st);
+    if (hd == 64) return launch_packed<64, false>(out, q, k, v, p, st);
+    return launch_packed<128, false>(out, q, k, v, p, st);
+}
 
 // The tensor-core prefill attention.  q / out [B*P x ld] (head h at columns
 // h*hd); keys and values of sequence b, head h at kc/vc + b*seq_stride +

@@ -68,6 +68,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // K-major, 128-byte-swizzled shared-memory operand descriptor: rows of 128
 // bytes, 8-row (1024-byte) swizzle atoms stacked with a 1024-byte stride.
 __device__ __forceinline__ uint64_t smem_desc(const void* tile, uint32_t byte_offset)
@@ -250,6 +259,22 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// The same, rounded to what kind::tf32 reads of it where ROUND (the unit cuts):
+// x is then hi + lo to 2^-22, without a bias, instead of 2^-21.
+template <bool ROUND>
+__device__ __forceinline__ float tf32_lo(float x)
+{
+    const float lo = x - tf32_hi(x);
+    return ROUND ? __uint_as_float(__float_as_uint(lo) + 0x1000u) : lo;
+}
+
+template <bool ROUND>
+__device__ __forceinline__ float4 tf32_lo4_as(const float4& x)
+{
+    if constexpr (!ROUND) return tf32_lo4(x);
+    return make_float4(tf32_lo<true>(x.x), tf32_lo<true>(x.y), tf32_lo<true>(x.z), tf32_lo<true>(x.w));
+}
+
 // ---- host side ---------------------------------------------------------------
 
 inline PFN_cuTensorMapEncodeTiled_v12000 get_encode()
@@ -282,6 +307,24 @@ inline int make_map(CUtensorMap* map, const float* base, int rows, int K, int ld
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(FML_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return FML_OK;
+}
+
+// [rows][heads][hd] fp32 (row stride ld floats) as BK x box_heads x box_rows
+// boxes with 128-byte swizzle: the rows of a box are its (row, head) pairs.
+inline int make_map_heads(CUtensorMap* map, const float* base, uint32_t hd, uint32_t heads, uint32_t rows, uint32_t ld,
+                          uint32_t box_heads, uint32_t box_rows)
+{
+    auto enc = get_encode();
+    if (!enc) return set_error(FML_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[3] = {hd, heads, rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * sizeof(float), (cuuint64_t)ld * sizeof(float)};
+    const cuuint32_t box[3] = {(cuuint32_t)BK, box_heads, box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(FML_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return FML_OK;
