@@ -159,7 +159,7 @@ def call(name: str, *args):
     """Call a status-returning entry point and raise on failure."""
     lib = load()
     rc = getattr(lib, name)(*args)
-    if SIGNATURES[name][0] is CHECKED_RESTYPE and name not in UNCHECKED and rc != FML_OK:
+    if rc != FML_OK and SIGNATURES[name][0] is CHECKED_RESTYPE and name not in UNCHECKED:
         raise FmlError(rc, name, lib.fml_last_error().decode(errors="replace"))
     return rc
 

@@ -68,53 +68,6 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// Four consecutive elements; VEC: one aligned access.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* p, float (&x)[4])
-{
-    if constexpr (VEC)
-    {
-        struct alignas(4 * sizeof(T)) Q
-        {
-            T e[4];
-        };
-        const Q q = *reinterpret_cast<const Q*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_f32(q.e[i]);
-    }
-    else
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_f32(p[i]);
-    }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T* p, const float (&x)[4])
-{
-    if constexpr (VEC)
-    {
-        struct alignas(4 * sizeof(T)) Q
-        {
-            T e[4];
-        } q;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q.e[i] = from_f32<T>(x[i]);
-        *reinterpret_cast<Q*>(p) = q;
-    }
-    else
-    {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = from_f32<T>(x[i]);
-    }
-}
-
 inline size_t type_bytes(int type) { return type == FML_TYPE_FP32 ? 4 : 2; }
-
-// Whether rows of `ld` elements from p can be read four elements at a time.
-inline bool vec4_ok(const void* p, uint32_t ld, int type)
-{
-    return reinterpret_cast<uintptr_t>(p) % (4 * type_bytes(type)) == 0 && ld % 4 == 0;
-}
 
 }  // namespace fml

@@ -1,10 +1,11 @@
 // The 4-bit paged key/value cache: rows written to it and read back, and the
 // page operations (reserve, fork, free, compact).
 //
-// Rows.  A thread has four consecutive columns of a row, eight neighbouring
-// threads a group of 32: the group's extremes are three shuffles.  A CTA takes
-// a run of tokens; its first warp finds each token's sequence (a binary search
-// in the starts), page and row once for all heads.
+// Rows.  A thread has eight consecutive columns of a key and of the value row,
+// four neighbouring threads a group of 32: the group's extremes are two
+// shuffles, and the eight key codes are one word.  A CTA takes a run of tokens;
+// its first threads find each token's sequence (a binary search in the starts),
+// page and row once for all heads.
 //
 // Pages.  Reference counts, tables and lengths are small integers; one CTA
 // settles them (block scans over the counts, in page order, so that the lowest
@@ -56,25 +57,27 @@ __device__ bool find_row(const Kv4View& c, const uint32_t* starts, uint32_t batc
     return true;
 }
 
-// Four values of a group as codes; the pair goes to every thread of the eight.
-__device__ __forceinline__ uint32_t quantise4(float (&x)[4], __half2* pair)
+// Eight values of a group as codes; the pair goes to every thread of the four.
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2* pair)
 {
     bool nan = false;
+    float lo = LIMIT, hi = -LIMIT;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
     {
         nan |= x[i] != x[i];
         x[i] = fminf(fmaxf(x[i], -LIMIT), LIMIT);
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
     }
-    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-    float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1)
+    for (int o = 1; o < 4; o <<= 1)
     {
         lo = fminf(lo, __shfl_xor_sync(FULL_MASK, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(FULL_MASK, hi, o));
-        nan |= __shfl_xor_sync(FULL_MASK, (int)nan, o) != 0;
     }
+    const uint32_t nans = __ballot_sync(FULL_MASK, nan);
+    nan = (nans >> (threadIdx.x & 28u) & 15u) != 0;
     const __half mn = __float2half_rn(lo);
     const float fm = __half2float(mn);
     const __half sc = __float2half_rn(__fmul_rn(hi - fm, 1.0f / 15.0f));
@@ -82,14 +85,59 @@ __device__ __forceinline__ uint32_t quantise4(float (&x)[4], __half2* pair)
     const float inv = fs == 0.0f ? 0.0f : __frcp_rn(fs);
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
     {
-        const float c = fminf(fmaxf(rintf(__fmul_rn(x[i] - fm, inv)), 0.0f), 15.0f);
-        codes |= (uint32_t)c << (4 * i);
+        // round to nearest, ties to even, clamped: as a whole number in the low bits
+        const float c = fminf(fmaxf(__fmul_rn(x[i] - fm, inv), 0.0f), 15.0f);
+        codes |= (__float_as_uint(c + 12582912.0f) & 15u) << (4 * i);
     }
     const __half bad = __ushort_as_half(0x7fff);
     *pair = nan ? __halves2half2(bad, bad) : __halves2half2(sc, mn);
     return nan ? 0u : codes;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8])
+{
+    if constexpr (VEC)
+    {
+        union
+        {
+            uint4 u[sizeof(T) / 2];
+            T e[8];
+        } q;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q.u[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(q.e[i]);
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8])
+{
+    if constexpr (VEC)
+    {
+        union
+        {
+            uint4 u[sizeof(T) / 2];
+            T e[8];
+        } q;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q.e[i] = from_f32<T>(x[i]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = q.u[i];
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(x[i]);
+    }
 }
 
 // READ false: rows of k and v become cache rows; true: the reverse.
@@ -98,7 +146,7 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
 {
     using B = Kv4Block<HD>;
     constexpr int NG = B::NG;
-    constexpr uint32_t UNITS = HD / 4;  // threads of a row
+    constexpr uint32_t UNITS = HD / 8;  // threads of a row
     __shared__ uint64_t at_s[MAX_TOKENS];
     __shared__ uint32_t row_s[MAX_TOKENS];
     const uint32_t page_size = 1u << a.c.page_shift, block = B::bytes(page_size);
@@ -113,47 +161,62 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
         row_s[threadIdx.x] = ok ? row : ~0u;
     }
     __syncthreads();
-    const uint32_t per_token = a.c.kv_heads * UNITS, total = 2 * n * per_token;
+    const uint32_t per_token = a.c.kv_heads * UNITS, total = n * per_token;
     for (uint32_t i0 = blockIdx.y * 256; i0 < total; i0 += gridDim.y * 256)
     {
-        const uint32_t i = i0 + threadIdx.x;
-        const bool in = i < total;
-        const uint32_t half = n * per_token;
-        const bool is_v = in && i >= half;
-        const uint32_t u = in ? (is_v ? i - half : i) : 0u;
+        const uint32_t i = i0 + threadIdx.x, u = i < total ? i : 0u;
         const uint32_t tok = u / per_token, hu = u - tok * per_token;
         const uint32_t head = hu / UNITS, lane = hu % UNITS;
         const uint32_t row = row_s[tok];
-        const bool live = in && row != ~0u;
-        T* src = (is_v ? a.v + (uint64_t)(r0 + tok) * a.ldv : a.k + (uint64_t)(r0 + tok) * a.ldk) + head * HD + 4 * lane;
-        unsigned char* blk = a.pool + at_s[tok] + (uint64_t)head * block + (is_v ? B::v(page_size) : 0u);
-        // key codes: word (lane / 2) of the row, its low or high half; value
-        // codes: two-byte unit (lane)
-        const uint32_t g = lane / 8, w = (lane & 7) >> 1, un = lane & 7;
-        const uint32_t unit = is_v ? un * NG + g : 2 * (w * NG + g) + (lane & 1);
-        uint16_t* code = reinterpret_cast<uint16_t*>(blk + row * B::ROW) + unit;
-        __half2* pair = reinterpret_cast<__half2*>(blk + B::kmeta(page_size) + row * B::META) + g;
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        const bool live = i < total && row != ~0u;
+        const uint32_t col = head * HD + 8 * lane;
+        T* k = a.k + (uint64_t)(r0 + tok) * a.ldk + col;
+        T* v = a.v + (uint64_t)(r0 + tok) * a.ldv + col;
+        unsigned char* blk = a.pool + at_s[tok] + (uint64_t)head * block;
+        // columns 32 g + 8 c ..: key word c * NG + g, value units 2 c * NG + g and (2 c + 1) * NG + g
+        const uint32_t g = lane / 4, c = lane & 3u, r = live ? row : 0u;
+        uint32_t* kw = reinterpret_cast<uint32_t*>(blk + r * B::ROW) + c * NG + g;
+        __half2* kp = reinterpret_cast<__half2*>(blk + B::kmeta(page_size) + r * B::META) + g;
+        uint16_t* vu = reinterpret_cast<uint16_t*>(blk + B::v(page_size) + r * B::ROW) + 2 * c * NG + g;
+        __half2* vp = reinterpret_cast<__half2*>(blk + B::vmeta(page_size) + r * B::META) + g;
+        float x[8], y[8];
         if constexpr (READ)
         {
             if (live)
             {
-                const uint32_t c = *code;
-                const float2 m = __half22float2(*pair);
+                const uint32_t kc = *kw, vc = vu[0] | (uint32_t)vu[NG] << 16;
+                const float2 km = __half22float2(*kp), vm = __half22float2(*vp);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fmaf((float)((c >> (4 * e)) & 15u), m.x, m.y);
-                store4<T, VEC>(src, x);
+                for (int e = 0; e < 8; ++e)
+                {
+                    x[e] = fmaf((float)((kc >> (4 * e)) & 15u), km.x, km.y);
+                    y[e] = fmaf((float)((vc >> (4 * e)) & 15u), vm.x, vm.y);
+                }
+                store8<T, VEC>(k, x);
+                store8<T, VEC>(v, y);
             }
         }
         else
         {
-            if (live) load4<T, VEC>(src, x);
-            __half2 m;
-            const uint32_t c = quantise4(x, &m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.f;
             if (live)
             {
-                *code = (uint16_t)c;
-                if ((lane & 7) == 0) *pair = m;
+                load8<T, VEC>(k, x);
+                load8<T, VEC>(v, y);
+            }
+            __half2 km, vm;
+            const uint32_t kc = quantise8(x, &km), vc = quantise8(y, &vm);
+            if (live)
+            {
+                *kw = kc;
+                vu[0] = (uint16_t)vc;
+                vu[NG] = (uint16_t)(vc >> 16);
+                if (c == 0)
+                {
+                    *kp = km;
+                    *vp = vm;
+                }
             }
         }
     }
@@ -163,9 +226,9 @@ template <typename T, int HD, bool READ>
 int launch_rows(const RowArgs<T>& a, bool vec, cudaStream_t st)
 {
     const uint32_t ctas = (a.rows + a.tokens - 1) / a.tokens;
-    const uint32_t units = 2 * min(a.tokens, a.rows) * a.c.kv_heads * (HD / 4);
-    uint32_t y = (units + 255) / 256;
-    if (y > 65535u) y = 65535u;
+    const uint64_t units = (uint64_t)(a.tokens < a.rows ? a.tokens : a.rows) * a.c.kv_heads * (HD / 8);
+    const uint64_t parts = (units + 1023) / 1024;  // CTAs that share a run of tokens: up to four passes each
+    const uint32_t y = (uint32_t)(parts < 65535u ? parts : 65535u);
     dim3 grid(ctas, y);
     if (vec) kv4_rows_kernel<T, HD, true, READ><<<grid, 256, 0, st>>>(a);
     else kv4_rows_kernel<T, HD, false, READ><<<grid, 256, 0, st>>>(a);
@@ -202,9 +265,9 @@ int rows_entry(const char* who, void* pool, const int32_t* table, const uint32_t
                 type);
     FML_REQUIRE((uint64_t)kv_heads * head_dim <= ldk && (uint64_t)kv_heads * head_dim <= ldv,
                 "%s: rows of %u heads of %u, strides %u and %u", who, kv_heads, head_dim, ldk, ldv);
-    const bool vec = vec4_ok(k, ldk, type) && vec4_ok(v, ldv, type);
+    const bool vec = aligned16(k) && aligned16(v) && (ldk | ldv) * type_bytes(type) % 16 == 0;
     // tokens of a CTA: as many as leave every SM a few CTAs
-    uint32_t tokens = rows / (148u * 8u);
+    uint32_t tokens = rows / (148u * 4u);
     tokens = tokens < 1 ? 1 : tokens > MAX_TOKENS ? MAX_TOKENS : tokens;
     const Kv4View c{table, lens, slot_ids, pages, slots, max_pages, kv4_page_shift(page_size), kv_heads};
     auto go = [&](auto* t) {

@@ -11,6 +11,8 @@ nothing.  `KV4Cache` keeps these tensors together.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from ._lib import FmlError, call, load
@@ -19,77 +21,101 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FML_TYPE_*
 NO_PAGES, BAD_SLOT, ROW_FULL = 1, 2, 4                           # FML_KV4_*
 
 
-def _check(cond, msg):
-    if not cond:
-        raise FmlError(1, "kv4", msg)
+def _refuse(msg):
+    raise FmlError(1, "kv4", msg)
 
 
-def _s():
-    return torch.cuda.current_stream().cuda_stream
+# The checks below run before every launch of a decode step: they are written
+# to cost little (the smallest calls take less time on the GPU than on the host).
+
+def _stream(t):
+    """The current stream of t's device, as the C ABI takes it."""
+    return _raw_stream(t.get_device())
+
+
+# torch.cuda.current_stream(device).cuda_stream builds a Stream object (3 us);
+# where torch has the plain query, that is used (0.1 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _rows(t, heads, hd, what):
     """(pointer, row stride) of [rows, heads, hd] whose heads are dense."""
-    s = t.stride()
-    if t.dim() != 3 or not t.is_cuda or t.shape[1] != heads or t.shape[2] != hd or s[2] != 1 or (s[1] != hd and heads > 1):
-        raise FmlError(1, "kv4", f"{what}: expected a CUDA tensor [rows, {heads}, {hd}] with dense heads")
-    return t.data_ptr(), max(s[0], heads * hd) if t.shape[0] < 2 else s[0]
+    if t.is_cuda and t.dim() == 3:
+        n, h, d = t.shape
+        s0, s1, s2 = t.stride()
+        if h == heads and d == hd and s2 == 1 and (s1 == hd or h == 1):
+            return t.data_ptr(), s0 if n > 1 else max(s0, h * d)
+    _refuse(f"{what}: expected a CUDA tensor [rows, {heads}, {hd}] with dense heads")
 
 
 def _ints(t, what, dims=1):
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or t.dim() != dims:
-        raise FmlError(1, "kv4", f"{what}: expected a contiguous int32 CUDA tensor of {dims} dimension(s)")
-    return t.data_ptr()
+    if t.dtype is torch.int32 and t.is_cuda and t.dim() == dims and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(f"{what}: expected a contiguous int32 CUDA tensor of {dims} dimension(s)")
 
 
 def _geometry(pool, hd):
     """(pages, kv_heads, page_size) of one layer's pool."""
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_cuda or not pool.is_contiguous() \
-            or pool.shape[3] * 4 != hd * 5:
-        raise FmlError(1, "kv4", f"pool: expected a contiguous uint8 CUDA tensor [pages, kv_heads, page_size, {hd * 5 // 4}]")
-    return pool.shape[:3]
+    if pool.dim() == 4 and pool.dtype is torch.uint8 and pool.is_cuda and pool.is_contiguous():
+        pages, heads, page, width = pool.shape
+        if width * 4 == hd * 5:
+            return pages, heads, page
+    _refuse(f"pool: expected a contiguous uint8 CUDA tensor [pages, kv_heads, page_size, {hd * 5 // 4}]")
+
+
+def _tables(table, lens, slot_ids, batch, what):
+    """(table, slots, max_pages, lens, slot_ids) as the C ABI takes them."""
+    at = _ints(table, "table", 2)
+    slots, most = table.shape
+    if lens.shape[0] != slots:
+        _refuse(f"{what}: lens of {lens.shape[0]} slots, a table of {slots}")
+    if slot_ids is None:
+        if batch > slots:
+            _refuse(f"{what}: {batch} entries, {slots} slots")
+    elif slot_ids.shape[0] != batch:
+        _refuse(f"{what}: {batch} entries, {slot_ids.shape[0]} slot_ids")
+    return at, slots, most, _ints(lens, "lens"), _ints(slot_ids, "slot_ids")
 
 
 def empty_pool(layers, pages, kv_heads, page_size, head_dim, device="cuda"):
     """Zeroed pools of `layers` layers."""
-    _check(int(load().fml_kv4_block_bytes(head_dim, page_size)) > 0, f"head_dim {head_dim}, page_size {page_size}")
+    if not int(load().fml_kv4_block_bytes(head_dim, page_size)):
+        _refuse(f"head_dim {head_dim}, page_size {page_size}")
     return torch.zeros(layers, pages, kv_heads, page_size, 5 * head_dim // 4, dtype=torch.uint8, device=device)
+
+
+def _new_rows(what, pool, table, lens, k, v, starts, slot_ids):
+    """The arguments that append and read share."""
+    hd = k.shape[-1]
+    pages, heads, page = _geometry(pool, hd)
+    pk, ldk = _rows(k, heads, hd, "k")
+    pv, ldv = _rows(v, heads, hd, "v")
+    kind, rows, batch = TYPES.get(k.dtype), k.shape[0], starts.shape[0] - 1
+    if kind is None or v.dtype is not k.dtype or v.shape[0] != rows:
+        _refuse(f"{what}: k and v differ, or their type")
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, what)
+    tail = (batch, rows, ldk, ldv, pages, slots, most, page, heads, hd, _stream(k))
+    return pool.data_ptr(), table, lens, slot_ids, pk, pv, kind, _ints(starts, "starts"), tail
 
 
 def append(pool, table, lens, k, v, starts, slot_ids=None):
     """Write each sequence's newest rows (fml_kv4_append): k, v [rows,
     kv_heads, hd]; rows starts[b] .. starts[b + 1] - 1 are entry b's last."""
-    hd = k.shape[-1]
-    pages, heads, page = _geometry(pool, hd)
-    pk, ldk = _rows(k, heads, hd, "k")
-    pv, ldv = _rows(v, heads, hd, "v")
-    _check(k.dtype == v.dtype and k.dtype in TYPES and k.shape[0] == v.shape[0], "append: k and v differ, or their type")
-    batch = starts.shape[0] - 1
-    _check(slot_ids is None and batch <= table.shape[0] or slot_ids is not None and slot_ids.shape[0] == batch,
-           "append: starts and slot_ids")
-    call("fml_kv4_append", pool.data_ptr(), _ints(table, "table", 2), _ints(lens, "lens"), _ints(slot_ids, "slot_ids"),
-         pk, pv, TYPES[k.dtype], _ints(starts, "starts"), batch, k.shape[0], ldk, ldv, pages, table.shape[0],
-         table.shape[1], page, heads, hd, _s())
+    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("append", pool, table, lens, k, v, starts, slot_ids)
+    call("fml_kv4_append", p, table, lens, slot_ids, pk, pv, kind, starts, *tail)
 
 
 def read(k, v, pool, table, lens, starts, slot_ids=None):
     """The values that each sequence's newest rows stand for, into k and v
     (fml_kv4_read); rows as in append."""
-    hd = k.shape[-1]
-    pages, heads, page = _geometry(pool, hd)
-    pk, ldk = _rows(k, heads, hd, "k")
-    pv, ldv = _rows(v, heads, hd, "v")
-    _check(k.dtype == v.dtype and k.dtype in TYPES and k.shape[0] == v.shape[0], "read: k and v differ, or their type")
-    batch = starts.shape[0] - 1
-    _check(slot_ids is None and batch <= table.shape[0] or slot_ids is not None and slot_ids.shape[0] == batch,
-           "read: starts and slot_ids")
-    call("fml_kv4_read", pk, pv, TYPES[k.dtype], pool.data_ptr(), _ints(table, "table", 2), _ints(lens, "lens"),
-         _ints(slot_ids, "slot_ids"), _ints(starts, "starts"), batch, k.shape[0], ldk, ldv, pages, table.shape[0],
-         table.shape[1], page, heads, hd, _s())
+    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("read", pool, table, lens, k, v, starts, slot_ids)
+    call("fml_kv4_read", pk, pv, kind, p, table, lens, slot_ids, starts, *tail)
 
 
+@lru_cache(maxsize=256)
 def attention_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_size):
     return int(load().fml_attention_kv4_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_size))
 
@@ -101,69 +127,82 @@ def attention(out, q, pool, table, lens, scale, slot_ids=None, workspace=None):
     pages, kv_heads, page = _geometry(pool, hd)
     pq, ldq = _rows(q, heads, hd, "q")
     po, ldo = _rows(out, heads, hd, "out")
-    _check(out.shape[0] == batch and out.dtype == q.dtype and q.dtype in TYPES, "attention: q and out differ, or their type")
-    _check(slot_ids is None and batch <= table.shape[0] or slot_ids is not None and slot_ids.shape[0] == batch,
-           "attention: batch and slot_ids")
-    slots, most = table.shape
-    need = attention_workspace_bytes(batch, heads, kv_heads, hd, most, page)
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    call("fml_attention_kv4", po, pq, TYPES[q.dtype], ldo, ldq, pool.data_ptr(), _ints(table, "table", 2),
-         _ints(lens, "lens"), _ints(slot_ids, "slot_ids"), batch, pages, slots, most, page, heads, kv_heads, hd,
-         float(scale), None if workspace is None else workspace.data_ptr(),
-         0 if workspace is None else workspace.numel() * workspace.element_size(), _s())
-
-
-def _pages_workspace(pages, n, device, workspace):
+    kind = TYPES.get(q.dtype)
+    if kind is None or out.dtype is not q.dtype or out.shape[0] != batch:
+        _refuse("attention: q and out differ, or their type")
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, "attention")
+    size, ws = 0, None
     if workspace is None:
-        workspace = torch.empty(int(load().fml_kv4_pages_workspace_bytes(pages, n)), dtype=torch.uint8, device=device)
+        size = attention_workspace_bytes(batch, heads, kv_heads, hd, most, page)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            ws = workspace.data_ptr()
+    else:
+        ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    call("fml_attention_kv4", po, pq, kind, ldo, ldq, pool.data_ptr(), table, lens, slot_ids, batch, pages, slots, most,
+         page, heads, kv_heads, hd, float(scale), ws, size, _stream(q))
+
+
+@lru_cache(maxsize=256)
+def _pages_bytes(pages, n):
+    return int(load().fml_kv4_pages_workspace_bytes(pages, n))
+
+
+def _pages_workspace(refs, n, workspace):
+    """(tensor, pointer, bytes); the tensor is held until the call is made."""
+    if workspace is None:
+        size = _pages_bytes(refs.shape[0], n)
+        workspace = torch.empty(size, dtype=torch.uint8, device=refs.device)
+        return workspace, workspace.data_ptr(), size
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _layers(pool):
-    if pool.dtype != torch.uint8 or pool.dim() != 5 or not pool.is_cuda or not pool.is_contiguous():
-        raise FmlError(1, "kv4", "pool: expected a contiguous uint8 CUDA tensor [layers, pages, kv_heads, page_size, bytes]")
-    page_bytes = pool.shape[2] * pool.shape[3] * pool.shape[4]
-    return pool.data_ptr(), pool.shape[0], pool.shape[1] * page_bytes, page_bytes
+def _layers(pool, pages):
+    """(pointer, layers, bytes from one to the next, bytes of a page, rows of a page)"""
+    if pool.dim() == 5 and pool.dtype is torch.uint8 and pool.is_cuda and pool.is_contiguous():
+        layers, n, heads, page, width = pool.shape
+        if n == pages:
+            return pool.data_ptr(), layers, n * heads * page * width, heads * page * width, page
+    _refuse(f"pool: expected a contiguous uint8 CUDA tensor [layers, {pages}, kv_heads, page_size, bytes]")
 
 
 def reserve(refs, table, lens, counts, page_size, status, slot_ids=None, workspace=None):
     """lens[slot] += counts[i], with pages for the new rows (fml_kv4_reserve)."""
     n, pages = counts.shape[0], refs.shape[0]
-    _check(slot_ids is None and n <= table.shape[0] or slot_ids is not None and slot_ids.shape[0] == n,
-           "reserve: counts and slot_ids")
-    ws, p, size = _pages_workspace(pages, max(n, 1), refs.device, workspace)
-    call("fml_kv4_reserve", _ints(refs, "refs"), _ints(table, "table", 2), _ints(lens, "lens"),
-         _ints(slot_ids, "slot_ids"), _ints(counts, "counts"), n, pages, table.shape[0], table.shape[1], page_size,
-         _ints(status, "status"), p, size, _s())
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "reserve")
+    hold, ws, size = _pages_workspace(refs, max(n, 1), workspace)
+    call("fml_kv4_reserve", _ints(refs, "refs"), table, lens, slot_ids, _ints(counts, "counts"), n, pages, slots, most,
+         page_size, _ints(status, "status"), ws, size, _stream(refs))
 
 
 def fork(pool, refs, table, lens, parents, children, status, workspace=None):
     """Slot children[i] becomes a copy of slot parents[i] (fml_kv4_fork): full
     pages shared, a page in use copied in every layer of pool."""
-    base, layers, stride, page_bytes = _layers(pool)
     n, pages = parents.shape[0], refs.shape[0]
-    _check(children.shape[0] == n and pool.shape[1] == pages, "fork: parents and children, or pool and refs")
-    ws, p, size = _pages_workspace(pages, max(n, 1), refs.device, workspace)
-    call("fml_kv4_fork", base, layers, stride, page_bytes, _ints(refs, "refs"), _ints(table, "table", 2),
-         _ints(lens, "lens"), _ints(parents, "parents"), _ints(children, "children"), n, pages, table.shape[0],
-         table.shape[1], pool.shape[3], _ints(status, "status"), p, size, _s())
+    base, layers, stride, page_bytes, page = _layers(pool, pages)
+    if children.shape[0] != n:
+        _refuse(f"fork: {n} parents, {children.shape[0]} children")
+    table, slots, most, lens, _ = _tables(table, lens, None, 0, "fork")
+    hold, ws, size = _pages_workspace(refs, max(n, 1), workspace)
+    call("fml_kv4_fork", base, layers, stride, page_bytes, _ints(refs, "refs"), table, lens, _ints(parents, "parents"),
+         _ints(children, "children"), n, pages, slots, most, page, _ints(status, "status"), ws, size, _stream(refs))
 
 
 def free(refs, table, lens, slot_ids, status):
     """Give the slots' pages back (fml_kv4_free)."""
-    call("fml_kv4_free", _ints(refs, "refs"), _ints(table, "table", 2), _ints(lens, "lens"), _ints(slot_ids, "slot_ids"),
-         slot_ids.shape[0], refs.shape[0], table.shape[0], table.shape[1], _ints(status, "status"), _s())
+    n = slot_ids.shape[0]
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "free")
+    call("fml_kv4_free", _ints(refs, "refs"), table, lens, slot_ids, n, refs.shape[0], slots, most,
+         _ints(status, "status"), _stream(refs))
 
 
 def compact(pool, refs, table, workspace=None):
     """Move the used pages together, in every layer of pool (fml_kv4_compact)."""
-    base, layers, stride, page_bytes = _layers(pool)
     pages = refs.shape[0]
-    _check(pool.shape[1] == pages, "compact: pool and refs")
-    ws, p, size = _pages_workspace(pages, 0, refs.device, workspace)
+    base, layers, stride, page_bytes, _ = _layers(pool, pages)
+    hold, ws, size = _pages_workspace(refs, 0, workspace)
     call("fml_kv4_compact", base, layers, stride, page_bytes, _ints(refs, "refs"), _ints(table, "table", 2), pages,
-         table.shape[0], table.shape[1], p, size, _s())
+         table.shape[0], table.shape[1], ws, size, _stream(refs))
 
 
 class KV4Cache:

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import torch
 
+from . import kv4
 from ._lib import FmlError, call
 
 NONE, RIGHT = 0, 1  # TransposeMode::None / TransposeMode::Right (MatrixBase_Mul.h:27)
@@ -144,21 +145,21 @@ def attention_packed(out, q, k, v, starts, scale, k_starts=None, mode=None):
     one QKV row will do); starts: int32 [batch + 1], the sequences' first rows;
     k_starts: the same for k and v where their rows lead the queries (a prompt
     run in chunks).  mode: FML_MATH_* of float32 (default: the library's)."""
-    from . import kv4
     heads, kv_heads, hd = q.shape[1], k.shape[1], q.shape[2]
     po, ldo = kv4._rows(out, heads, hd, "out")
     pq, ldq = kv4._rows(q, heads, hd, "q")
     pk, ldk = kv4._rows(k, kv_heads, hd, "k")
     pv, ldv = kv4._rows(v, kv_heads, hd, "v")
-    _check(q.dtype in kv4.TYPES and out.dtype == k.dtype == v.dtype == q.dtype, "attention_packed types")
-    _check(out.shape[0] == q.shape[0] and k.shape[0] == v.shape[0] and
-           (k_starts is None or k_starts.shape == starts.shape), "attention_packed shapes")
+    kind, rows, k_rows, n = kv4.TYPES.get(q.dtype), q.shape[0], k.shape[0], starts.shape[0]
+    if kind is None or out.dtype is not q.dtype or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise FmlError(1, "matrix_ops", "attention_packed types")
+    if out.shape[0] != rows or v.shape[0] != k_rows or (k_starts is None and k_rows != rows) or \
+            (k_starts is not None and k_starts.shape[0] != n):
+        raise FmlError(1, "matrix_ops", "attention_packed shapes")
     if mode is None:
-        from ._lib import load
-        mode = int(load().fml_get_math_mode())
-    call("fml_attention_packed", po, pq, pk, pv, kv4.TYPES[q.dtype], kv4._ints(starts, "starts"),
-         kv4._ints(k_starts, "k_starts"), starts.shape[0] - 1, q.shape[0], k.shape[0], heads, kv_heads, hd, ldo, ldq, ldk,
-         ldv, float(scale), int(mode), _s())
+        mode = call("fml_get_math_mode")
+    call("fml_attention_packed", po, pq, pk, pv, kind, kv4._ints(starts, "starts"), kv4._ints(k_starts, "k_starts"),
+         n - 1, rows, k_rows, heads, kv_heads, hd, ldo, ldq, ldk, ldv, float(scale), mode, kv4._stream(q))
 
 
 def attention_decode(out, q, kcache, vcache, lens, scale, workspace=None):
