@@ -643,38 +643,51 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     }
 }
 
-// Joins the segments of split sequences: one warp per (entry, query head).
+// Joins the segments of split sequences: one CTA per (entry, query head), whose
+// warps take the segments in turn (a warp alone waits for one segment after
+// another: 10 us for 50 of them, against 3).
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) kv4_join_kernel(Kv4AttnArgs<T> a, uint32_t chunks)
+__global__ void __launch_bounds__(32 * NW) kv4_join_kernel(Kv4AttnArgs<T> a, uint32_t chunks)
 {
-    const uint32_t lane = threadIdx.x & 31u, w = blockIdx.x * 4 + (threadIdx.x >> 5);
+    constexpr int E = HD / 32;
+    __shared__ float sum_s[NW], o_s[NW][HD];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, kvh = h / a.group, g = h % a.group;
     griddep_wait();
-    if (w >= a.batch * a.heads) return;
-    const uint32_t b = w / a.heads, h = w % a.heads, kvh = h / a.group, g = h % a.group;
     const uint2 at = a.where[b];
     if (at.y <= 1) return;
     const uint64_t step = (uint64_t)a.c.kv_heads * chunks * GQ * (HD + 2);
-    const float* p = a.partial + (uint64_t)at.x * step +
-                     (((uint64_t)kvh * chunks + g / GQ) * GQ + g % GQ) * (HD + 2);
+    const float* p = a.partial + (uint64_t)at.x * step + (((uint64_t)kvh * chunks + g / GQ) * GQ + g % GQ) * (HD + 2);
     float top = -INFINITY;
     for (uint32_t s = lane; s < at.y; s += 32) top = fmaxf(top, p[s * step]);
     top = warp_max(top);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o[HD / 32];
+    float sum = 0.f, o[E];
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) o[e] = 0.f;
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll 4
-    for (uint32_t s = 0; s < at.y; ++s)
+    for (uint32_t s = warp; s < at.y; s += NW)
     {
         const float* r = p + s * step;
         const float f = ex2(r[0] - base);
         sum = fmaf(r[1], f, sum);
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) o[e] = fmaf(r[2 + 32 * e + lane], f, o[e]);
+        for (int e = 0; e < E; ++e) o[e] = fmaf(r[2 + 32 * e + lane], f, o[e]);
     }
+    if (lane == 0) sum_s[warp] = sum;
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e)
-        a.out[(uint64_t)b * a.ldo + h * HD + 32 * e + lane] = from_f32<T>(sum == 0.f ? 0.f : o[e] / sum);
+    for (int e = 0; e < E; ++e) o_s[warp][32 * e + lane] = o[e];
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += sum_s[w];
+    for (uint32_t d = threadIdx.x; d < HD; d += 32 * NW)
+    {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += o_s[w][d];
+        a.out[(uint64_t)b * a.ldo + h * HD + d] = from_f32<T>(sum == 0.f ? 0.f : x / sum);
+    }
 }
 
 // Segments that one head's keys are cut into, about, and their bound.
@@ -712,8 +725,8 @@ int launch(const Kv4AttnArgs<T>& a, const Split& s, cudaStream_t st)
     FML_LAUNCH_CHECK();
     if (!s.split) return FML_OK;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(((uint64_t)a.batch * a.heads + 3) / 4));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(a.batch * a.heads);
+    cfg.blockDim = dim3(32 * NW);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

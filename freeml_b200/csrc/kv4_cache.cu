@@ -152,6 +152,15 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
     const uint32_t page_size = 1u << a.c.page_shift, block = B::bytes(page_size);
     const uint32_t r0 = blockIdx.x * a.tokens;
     const uint32_t n = min(a.tokens, a.rows - r0);
+    const uint32_t per_token = a.c.kv_heads * UNITS, total = n * per_token;
+    // the values of the first pass are on their way while the rows are found
+    float x[8], y[8];
+    auto fetch = [&](uint32_t i) {
+        const uint32_t u = i < total ? i : 0u, tok = u / per_token, col = (u - tok * per_token) * 8;
+        load8<T, VEC>(a.k + (uint64_t)(r0 + tok) * a.ldk + col, x);
+        load8<T, VEC>(a.v + (uint64_t)(r0 + tok) * a.ldv + col, y);
+    };
+    if constexpr (!READ) fetch(blockIdx.y * 256 + threadIdx.x);
     if (threadIdx.x < n)
     {
         uint64_t at = 0;
@@ -161,7 +170,6 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
         row_s[threadIdx.x] = ok ? row : ~0u;
     }
     __syncthreads();
-    const uint32_t per_token = a.c.kv_heads * UNITS, total = n * per_token;
     for (uint32_t i0 = blockIdx.y * 256; i0 < total; i0 += gridDim.y * 256)
     {
         const uint32_t i = i0 + threadIdx.x, u = i < total ? i : 0u;
@@ -170,8 +178,6 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
         const uint32_t row = row_s[tok];
         const bool live = i < total && row != ~0u;
         const uint32_t col = head * HD + 8 * lane;
-        T* k = a.k + (uint64_t)(r0 + tok) * a.ldk + col;
-        T* v = a.v + (uint64_t)(r0 + tok) * a.ldv + col;
         unsigned char* blk = a.pool + at_s[tok] + (uint64_t)head * block;
         // columns 32 g + 8 c ..: key word c * NG + g, value units 2 c * NG + g and (2 c + 1) * NG + g
         const uint32_t g = lane / 4, c = lane & 3u, r = live ? row : 0u;
@@ -179,7 +185,6 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
         __half2* kp = reinterpret_cast<__half2*>(blk + B::kmeta(page_size) + r * B::META) + g;
         uint16_t* vu = reinterpret_cast<uint16_t*>(blk + B::v(page_size) + r * B::ROW) + 2 * c * NG + g;
         __half2* vp = reinterpret_cast<__half2*>(blk + B::vmeta(page_size) + r * B::META) + g;
-        float x[8], y[8];
         if constexpr (READ)
         {
             if (live)
@@ -192,21 +197,15 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
                     x[e] = fmaf((float)((kc >> (4 * e)) & 15u), km.x, km.y);
                     y[e] = fmaf((float)((vc >> (4 * e)) & 15u), vm.x, vm.y);
                 }
-                store8<T, VEC>(k, x);
-                store8<T, VEC>(v, y);
+                store8<T, VEC>(a.k + (uint64_t)(r0 + tok) * a.ldk + col, x);
+                store8<T, VEC>(a.v + (uint64_t)(r0 + tok) * a.ldv + col, y);
             }
         }
         else
         {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.f;
-            if (live)
-            {
-                load8<T, VEC>(k, x);
-                load8<T, VEC>(v, y);
-            }
             __half2 km, vm;
             const uint32_t kc = quantise8(x, &km), vc = quantise8(y, &vm);
+            if (i0 + gridDim.y * 256 < total) fetch(i + gridDim.y * 256);
             if (live)
             {
                 *kw = kc;
@@ -267,7 +266,7 @@ int rows_entry(const char* who, void* pool, const int32_t* table, const uint32_t
                 "%s: rows of %u heads of %u, strides %u and %u", who, kv_heads, head_dim, ldk, ldv);
     const bool vec = aligned16(k) && aligned16(v) && (ldk | ldv) * type_bytes(type) % 16 == 0;
     // tokens of a CTA: as many as leave every SM a few CTAs
-    uint32_t tokens = rows / (148u * 4u);
+    uint32_t tokens = rows / (148u * 16u);
     tokens = tokens < 1 ? 1 : tokens > MAX_TOKENS ? MAX_TOKENS : tokens;
     const Kv4View c{table, lens, slot_ids, pages, slots, max_pages, kv4_page_shift(page_size), kv_heads};
     auto go = [&](auto* t) {
