@@ -5,8 +5,8 @@
 //
 // CTA = 4 warps on (128 query rows, head, sequence); it walks the key tiles
 // (KT keys) up to its last row.  Per tile:
-//   1. K tile (TMA, 128-byte swizzle, K-major) -> its TF32 lo part; one
-//      thread issues S = Q K^T (Q_hi K_hi + Q_hi K_lo + Q_lo K_hi) into TMEM;
+//   1. K tile (TMA, 128-byte swizzle, K-major) -> its TF32 lo part; the first
+//      warp issues S = Q K^T (Q_hi K_hi + Q_hi K_lo + Q_lo K_hi) into TMEM;
 //   2. thread r (= TMEM lane r) reads query row r's KT scores with
 //      tcgen05.ld, scales and masks them (keys past the row and past the
 //      prompt), and updates the row's online softmax (running max m and sum
@@ -15,7 +15,7 @@
 //   3. V tile: TMA in the 128-byte swizzle of 32-byte atoms, the layout an
 //      N-major tf32 operand needs (V is stored [keys x hd], hd contiguous);
 //      rows past the last valid key are zeroed (the cache may hold anything
-//      there); one thread issues O_tile = P V (TF32x3) into a second TMEM
+//      there); the first warp issues O_tile = P V (TF32x3) into a second TMEM
 //      accumulator;
 //   4. thread r reads its O_tile row and accumulates O = O corr + O_tile in
 //      registers (corr = exp(m_old - m_new)).
@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(FULL_MASK, *tmem_slot, 0);  // the same in the warp for the compiler too
+    const bool warp0 = __shfl_sync(FULL_MASK, warp, 0) == 0;
     const uint32_t tmem_o = tmem + Sh::OCOL;
     const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
 
@@ -212,22 +213,23 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         ok = __syncthreads_and(ok) != 0;
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (tid == 0)
+        if (warp0)
         {
+#pragma unroll
             for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
                 {
                     const uint64_t da = smem_desc(q_s + j * (QB * 128), kk * 32);
                     const uint64_t db = smem_desc(k_s + j * (KT * 128), kk * 32);
-                    mma_tf32(tmem, da, db, IDESC_S, j > 0 || kk > 0);
+                    mma_tf32_elected(tmem, da, db, IDESC_S, j > 0 || kk > 0);
                     if constexpr (SPLIT3)
                     {
-                        mma_tf32(tmem, da, smem_desc(klo_s + j * (KT * 128), kk * 32), IDESC_S, true);
-                        mma_tf32(tmem, smem_desc(qlo_s + j * (QB * 128), kk * 32), db, IDESC_S, true);
+                        mma_tf32_elected(tmem, da, smem_desc(klo_s + j * (KT * 128), kk * 32), IDESC_S, true);
+                        mma_tf32_elected(tmem, smem_desc(qlo_s + j * (QB * 128), kk * 32), db, IDESC_S, true);
                     }
                 }
-            mma_commit(&bars[BS]);
+            mma_commit_elected(&bars[BS]);
             ++issued[BS];
         }
         ok = wait(BS, t);
@@ -317,22 +319,23 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         ok = __syncthreads_and(ok) != 0;
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (tid == 0)
+        if (warp0)
         {
+#pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
                 {
                     const uint64_t da = smem_desc(p_s + kb * (QB * 128), kk * 32);
                     const uint64_t db = desc_mn(v_s + kb * (HD / 32) * 4096 + kk * 1024);
-                    mma_tf32(tmem_o, da, db, IDESC_O, kb > 0 || kk > 0);
+                    mma_tf32_elected(tmem_o, da, db, IDESC_O, kb > 0 || kk > 0);
                     if constexpr (SPLIT3)
                     {
-                        mma_tf32(tmem_o, da, desc_mn(vlo_s + kb * (HD / 32) * 4096 + kk * 1024), IDESC_O, true);
-                        mma_tf32(tmem_o, smem_desc(plo_s + kb * (QB * 128), kk * 32), db, IDESC_O, true);
+                        mma_tf32_elected(tmem_o, da, desc_mn(vlo_s + kb * (HD / 32) * 4096 + kk * 1024), IDESC_O, true);
+                        mma_tf32_elected(tmem_o, smem_desc(plo_s + kb * (QB * 128), kk * 32), db, IDESC_O, true);
                     }
                 }
-            mma_commit(&bars[BO]);
+            mma_commit_elected(&bars[BO]);
             ++issued[BO];
         }
         ok = wait(BO, t);
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 //   warps 4-7   softmax of tile B
 //   warp 8      converter: the TF32 lo parts of K and V (TF32x3) and the
 //               zeroing of V rows past the last key any row sees
-//   warps 9-10  one thread each issues tile A's / tile B's tcgen05.mma
+//   warps 9-10  tile A's / tile B's tcgen05.mma (one lane elected)
 //   warp 11     one thread issues every TMA copy
 // K and V operand tiles are double-buffered: the copy and the conversion of
 // key tile t + 1 run while tile t's products do.
@@ -408,9 +411,9 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 // on the reference maximum.
 // The tensor pipe's instruction queue is short: while the thread that issues
 // MMAs waits on an mbarrier (even one already complete, ~170 cycles), the
-// pipe drains and idles.  So each query tile has its own issuing thread, in
-// its own warp, and the pipe runs one tile's products while the other's
-// thread waits (for its softmax, or for the completion of O_x(t-1): S_x(t)
+// pipe drains and idles.  So each query tile has its own issuing warp, and
+// the pipe runs one tile's products while the other's
+// warp waits (for its softmax, or for the completion of O_x(t-1): S_x(t)
 // overwrites the columns P_x(t-1) is read from).
 // Every wait is bounded and also returns early once any role has recorded an
 // expiry in the CTA's abort flag; the MMA thread then waits for its MMAs and
@@ -765,22 +768,23 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     else if (warp < 11)
     {
         // ---------------- MMA issue for tile x ----------------
-        const int x = warp - 9;
+        const int x = __shfl_sync(FULL_MASK, warp, 0) - 9;  // the same in the warp for the compiler too
         const uint32_t nt = x ? nt1 : nt0;
-        if (lane == 0 && nt > 0)
+        if (nt > 0)
         {
+            auto wait = [&](int i, uint32_t ph) { return __all_sync(FULL_MASK, mbar_wait_or(&bars[i], ph, abort)) != 0; };
             // descriptors: one base each, advanced by (byte offset >> 4) in
             // the start-address field (shared addresses stay below 2^18)
             const uint64_t dq = smem_desc(q_s + x * PP_QTILE, 0);
             const uint64_t dk = smem_desc(k_op, 0), dv = desc_mn(v_op);
             const uint32_t ts = tmem + PP_TX * x, to = ts + PP_O;
-            bool ok = mbar_wait_or(&bars[PB_QR], 0, abort);
+            bool ok = wait(PB_QR, 0);
             for (uint32_t t = 0; ok && t < nt; ++t)
             {
                 const uint32_t bf = t & 1u, ph = t >> 1;
                 // S_x(t) = Q_x K(t)^T, after O_x(t-1) has read P_x(t-1)
-                if (!(ok = mbar_wait_or(&bars[PB_KR + bf], ph, abort))) break;
-                if (t > 0 && !(ok = mbar_wait_or(&bars[PB_O0 + x], t - 1, abort))) break;
+                if (!(ok = wait(PB_KR + bf, ph))) break;
+                if (t > 0 && !(ok = wait(PB_O0 + x, t - 1))) break;
                 tc_fence_after();
                 const uint64_t kbase = dk + ((bf * PP_KVOP) >> 4);
 #pragma unroll
@@ -793,17 +797,17 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                         if constexpr (SPLIT3)
                         {
                             // [hi.hi | hi.lo] in one MMA, then lo.hi (Q lo from TMEM) into the first half
-                            mma_tf32(ts, da, db, IDESC_S2, j > 0 || kk > 0);
-                            mma_tf32_tmem_a(ts, ts + PP_QLO + 32 * j + 8 * kk, db, IDESC_S, true);
+                            mma_tf32_elected(ts, da, db, IDESC_S2, j > 0 || kk > 0);
+                            mma_tf32_tmem_a_elected(ts, ts + PP_QLO + 32 * j + 8 * kk, db, IDESC_S, true);
                         }
                         else
-                            mma_tf32(ts, da, db, IDESC_S, j > 0 || kk > 0);
+                            mma_tf32_elected(ts, da, db, IDESC_S, j > 0 || kk > 0);
                     }
-                mma_commit(&bars[PB_S0 + x]);
-                mma_commit(&bars[PB_KE + 2 * x + bf]);
+                mma_commit_elected(&bars[PB_S0 + x]);
+                mma_commit_elected(&bars[PB_KE + 2 * x + bf]);
                 // O_x += P_x(t) V(t)
-                if (!(ok = mbar_wait_or(&bars[PB_VR + bf], ph, abort))) break;
-                if (!(ok = mbar_wait_or(&bars[PB_P0 + x], t, abort))) break;
+                if (!(ok = wait(PB_VR + bf, ph))) break;
+                if (!(ok = wait(PB_P0 + x, t))) break;
                 tc_fence_after();
                 const uint64_t vbase = dv + ((bf * PP_KVOP) >> 4);
 #pragma unroll
@@ -813,19 +817,19 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                     {
                         const uint64_t db = vbase + ((kb * PP_VBLK + kk * 1024) >> 4);
                         const uint32_t col = kb * 32 + kk * 8;
-                        mma_tf32_tmem_a(to, ts + col, db, IDESC_O, t > 0 || kb > 0 || kk > 0);
+                        mma_tf32_tmem_a_elected(to, ts + col, db, IDESC_O, t > 0 || kb > 0 || kk > 0);
                         if constexpr (SPLIT3)
                         {
-                            mma_tf32_tmem_a(to, ts + col, db + (8192 >> 4), IDESC_O, true);  // P hi . V lo
-                            mma_tf32_tmem_a(to, ts + PP_PLO + col, db, IDESC_O, true);      // P lo . V hi
+                            mma_tf32_tmem_a_elected(to, ts + col, db + (8192 >> 4), IDESC_O, true);  // P hi . V lo
+                            mma_tf32_tmem_a_elected(to, ts + PP_PLO + col, db, IDESC_O, true);      // P lo . V hi
                         }
                     }
-                mma_commit(&bars[PB_O0 + x]);
-                mma_commit(&bars[PB_VE + 2 * x + bf]);
+                mma_commit_elected(&bars[PB_O0 + x]);
+                mma_commit_elected(&bars[PB_VE + 2 * x + bf]);
             }
-            // every MMA this thread issued completes before TMEM is freed
-            mma_commit(&bars[PB_FIN + x]);
-            mbar_wait(&bars[PB_FIN + x], 0);
+            // every MMA this warp issued completes before TMEM is freed
+            mma_commit_elected(&bars[PB_FIN + x]);
+            __all_sync(FULL_MASK, mbar_wait(&bars[PB_FIN + x], 0));
         }
     }
     else

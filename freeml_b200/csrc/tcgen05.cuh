@@ -119,6 +119,43 @@ __device__ __forceinline__ void mma_tf32_tmem_a(uint32_t tmem_d, uint32_t tmem_a
         : "memory");
 }
 
+// The same three from a whole warp, of which the hardware elects one lane (the
+// same one each time): operands are then the same in the warp for the compiler
+// too.  From a branch of one thread a product takes 80 to 130 cycles to issue,
+// more than a small one takes to run; so, 15 to 25.
+__device__ __forceinline__ void mma_tf32_elected(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                                 bool accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_tf32_tmem_a_elected(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
+                                                        bool accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_commit_elected(uint64_t* bar)
+{
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+
 // Arrive on `bar` once every tcgen05.mma this thread issued has completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar)
 {
