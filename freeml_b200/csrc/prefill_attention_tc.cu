@@ -23,10 +23,6 @@
 // start as soon as the MMAs that read the current ones have completed.
 // Every mbarrier wait is bounded (expiries are counted in the device error
 // count; the CTA then stops issuing work and still frees its TMEM).
-//
-// PACKED: the same over packed prompts with grouped heads (packed.cuh): the
-// CTA's rows are (token, query head) pairs of one key/value head, each with the
-// number of keys that it sees.
 #include <cmath>
 #include <cstdlib>
 
@@ -62,10 +58,9 @@ struct PfShape
     static constexpr uint32_t TCOLS = OCOL + HD <= 128 ? 128 : 256;
 };
 
-template <bool ROUND>
 __device__ __forceinline__ void lo_inplace(float4* dst, const float4* src, uint32_t n4, int tid)
 {
-    for (uint32_t i = tid; i < n4; i += 128) dst[i] = tc::tf32_lo4_as<ROUND>(src[i]);
+    for (uint32_t i = tid; i < n4; i += 128) dst[i] = tc::tf32_lo4(src[i]);
 }
 
 __device__ __forceinline__ uint64_t desc_mn(const void* tile)
@@ -78,11 +73,11 @@ __device__ __forceinline__ uint64_t desc_mn(const void* tile)
 
 }  // namespace
 
-template <int HD, bool SPLIT3, bool PACKED>
+template <int HD, bool SPLIT3>
 __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                       const __grid_constant__ CUtensorMap map_k,
                                                                       const __grid_constant__ CUtensorMap map_v,
-                                                                      PfArgs a, PackedArgs pk)
+                                                                      PfArgs a)
 {
     using namespace tc;
     using Sh = PfShape<HD>;
@@ -106,29 +101,12 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     enum { BQ = 0, BKEY = 1, BVAL = 2, BS = 3, BO = 4 };
 
     const int tid = threadIdx.x, warp = tid >> 5;
-    const uint32_t q0 = PACKED ? 0u : blockIdx.x * QB, h = blockIdx.y, b = blockIdx.z;
+    const uint32_t q0 = blockIdx.x * QB, h = blockIdx.y, b = blockIdx.z;
     const uint32_t P = a.P;
-    uint32_t nkeys = min(q0 + (uint32_t)QB, P);               // keys this CTA's rows can see
-    int kv_row0 = (int)((b * a.H + h) * a.C), kv_col0 = 0;    // this (sequence, head)'s first cache row
-    const uint32_t q = q0 + tid;                              // this thread's query row
-    uint32_t sees = 0, q_row = b * P + q, q_head = h;         // PACKED: keys it sees; its place in q and out
-    bool live = q < P;
-    PackedTile pt{};
-    if constexpr (PACKED)
-    {
-        pt = packed_tile<128>(pk, blockIdx.x);
-        if (!pt.live) return;
-        const uint32_t kvh = h / pk.nchunk, hc = (h % pk.nchunk) * pk.gs, tok = tid / pk.gs, head = tid % pk.gs;
-        const uint32_t tokens = min(pk.tpt, pt.lq - pt.t0);
-        live = tok < tokens && head < min(pk.gs, pk.group - hc);
-        nkeys = keys_seen(pt, pt.t0 + tokens - 1);
-        sees = live ? keys_seen(pt, pt.t0 + tok) : 0u;
-        kv_row0 = (int)pt.k0;
-        kv_col0 = (int)(kvh * HD);
-        q_row = pt.q0 + pt.t0 + tok;
-        q_head = kvh * pk.group + hc + head;
-    }
+    const uint32_t nkeys = min(q0 + (uint32_t)QB, P);         // keys this CTA's rows can see
     const uint32_t ntiles = (nkeys + KT - 1) / KT;
+    const int kv_row0 = (int)((b * a.H + h) * a.C);           // this (sequence, head)'s first cache row
+    const uint32_t q = q0 + tid;                              // this thread's query row
     // thread 0's count of the phases it started / saw complete on each barrier
     // (the drain after an expired wait)
     uint32_t issued[5] = {0, 0, 0, 0, 0}, seen[5] = {0, 0, 0, 0, 0};
@@ -156,15 +134,15 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     auto issue_k = [&](uint32_t t) {
         mbar_arrive_expect_tx(&bars[BKEY], Sh::KBYTES);
         for (int j = 0; j < HD / 32; ++j)
-            tma_load_2d(k_s + j * (KT * 128), &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * KT), &bars[BKEY]);
+            tma_load_2d(k_s + j * (KT * 128), &map_k, 32 * j, kv_row0 + (int)(t * KT), &bars[BKEY]);
         ++issued[BKEY];
     };
     auto issue_v = [&](uint32_t t) {
         mbar_arrive_expect_tx(&bars[BVAL], Sh::VBYTES);
         for (int kb = 0; kb < KT / 32; ++kb)
             for (int j = 0; j < HD / 32; ++j)
-                tma_load_2d(v_s + (kb * (HD / 32) + j) * 4096, &map_v, kv_col0 + 32 * j,
-                            kv_row0 + (int)(t * KT) + 32 * kb, &bars[BVAL]);
+                tma_load_2d(v_s + (kb * (HD / 32) + j) * 4096, &map_v, 32 * j, kv_row0 + (int)(t * KT) + 32 * kb,
+                            &bars[BVAL]);
         ++issued[BVAL];
     };
     // bounded wait on phase `ph` of barrier i, the same answer in the whole warp
@@ -175,24 +153,18 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     };
     if (tid == 0)
     {
-        mbar_arrive_expect_tx(&bars[BQ], PACKED ? (HD / 32) * pk.gs * pk.tpt * 128 : Sh::QBYTES);
+        mbar_arrive_expect_tx(&bars[BQ], Sh::QBYTES);
         for (int j = 0; j < HD / 32; ++j)
-            if constexpr (PACKED)  // thread 0's row is the tile's first
-                tma_load_3d(q_s + j * (QB * 128), &map_q, 32 * j, (int)q_head, (int)q_row, &bars[BQ]);
-            else
-                tma_load_2d(q_s + j * (QB * 128), &map_q, (int)(h * HD) + 32 * j, (int)(b * P + q0), &bars[BQ]);
+            tma_load_2d(q_s + j * (QB * 128), &map_q, (int)(h * HD) + 32 * j, (int)(b * P + q0), &bars[BQ]);
         issued[BQ] = 1;
-        if (!PACKED || ntiles > 0)
-        {
-            issue_k(0);
-            issue_v(0);
-        }
+        issue_k(0);
+        issue_v(0);
     }
 
     bool ok = wait(BQ, 0);
     if constexpr (SPLIT3)
         if (ok)
-            lo_inplace<PACKED>(reinterpret_cast<float4*>(qlo_s), reinterpret_cast<const float4*>(q_s), Sh::QBYTES / 16, tid);
+            lo_inplace(reinterpret_cast<float4*>(qlo_s), reinterpret_cast<const float4*>(q_s), Sh::QBYTES / 16, tid);
 
     float o[HD];
 #pragma unroll
@@ -206,7 +178,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         if (ok) ok = wait(BKEY, t);
         if constexpr (SPLIT3)
             if (ok)
-                lo_inplace<PACKED>(reinterpret_cast<float4*>(klo_s), reinterpret_cast<const float4*>(k_s), Sh::KBYTES / 16,
+                lo_inplace(reinterpret_cast<float4*>(klo_s), reinterpret_cast<const float4*>(k_s), Sh::KBYTES / 16,
                            tid);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -260,8 +232,8 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
         for (int i = 0; i < KT; ++i)
         {
             const uint32_t key = k0 + i;
-            const bool in = PACKED ? key < sees : key <= q && key < P;
-            sv[i] = in ? sv[i] * a.scale : -INFINITY;  // a select: masked slots may hold anything
+            const bool live = key <= q && key < P;
+            sv[i] = live ? sv[i] * a.scale : -INFINITY;  // a select: masked slots may hold anything
             mx = fmaxf(mx, sv[i]);
         }
         const float corr = m == -INFINITY ? 0.f : expf(m - mx);
@@ -285,7 +257,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
                                               sv[kb * 32 + 4 * c + 3]);
                 const uint32_t off = kb * (QB * 128) + tid * 128 + ((c ^ (tid & 7)) * 16);
                 *reinterpret_cast<float4*>(p_s + off) = pv;
-                if constexpr (SPLIT3) *reinterpret_cast<float4*>(plo_s + off) = tf32_lo4_as<PACKED>(pv);
+                if constexpr (SPLIT3) *reinterpret_cast<float4*>(plo_s + off) = tf32_lo4(pv);
             }
 
         // ---- O_tile = P V ----
@@ -310,7 +282,7 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
                         if constexpr (SPLIT3) vlo4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     }
                     else if constexpr (SPLIT3)
-                        vlo4[i] = tf32_lo4_as<PACKED>(v4[i]);
+                        vlo4[i] = tf32_lo4(v4[i]);
                 }
             }
         }
@@ -356,11 +328,10 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
     }
     ok = __syncthreads_and(ok) != 0;
 
-    if (ok && live)
+    if (ok && q < P)
     {
-        // l >= 1: the row's largest score contributes exp(0); a packed row may see no key
-        const float inv = PACKED && sees == 0 ? 0.f : 1.0f / l;
-        float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
+        const float inv = 1.0f / l;  // l >= 1: the row's largest score contributes exp(0)
+        float* dst = a.out + (uint64_t)(b * P + q) * a.ldo + h * HD;
 #pragma unroll
         for (int e = 0; e < HD; e += 4)
             *reinterpret_cast<float4*>(dst + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
@@ -415,50 +386,70 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 // the pipe runs one tile's products while the other's
 // warp waits (for its softmax, or for the completion of O_x(t-1): S_x(t)
 // overwrites the columns P_x(t-1) is read from).
+//
+// PACKED: the same over packed prompts with grouped heads (packed.cuh) at head
+// dims 32, 64 and 128: the CTA's rows are (token, query head) pairs of one
+// key/value head, each with the number of keys that it sees.  The remainders
+// are rounded to TF32 there (the product truncates them otherwise, which
+// doubles the error), and head dim 128 runs one query tile and one buffer of
+// K and V (PpShape).  Bound by the tensor pipe's three TF32 products and by the
+// softmax warps' time between them.  Measured on a B200, one causal prompt of
+// 512 tokens: 4 heads of 32 25 us, 8 of 64 32 us, 32 on 8 of 128 35 us (one
+// tile with S and P V through registers, the first kernel's way: 48, 61, 91 us;
+// CUDA cores: 43, 61, 151 us); 64 ragged prompts of 1 to 512 tokens, 8 heads of
+// 64: 48 us.
 // Every wait is bounded and also returns early once any role has recorded an
 // expiry in the CTA's abort flag; the MMA thread then waits for its MMAs and
 // the copy thread for its copies (bounded) before TMEM is freed.
 namespace {
 
-constexpr int PP_HD = 64, PP_KT = 64;
-constexpr uint32_t PP_QTILE = 128 * PP_HD * 4;  // one 128-row Q tile, 32 KB
-constexpr uint32_t PP_KVT = PP_KT * PP_HD * 4;  // one K or V tile, 16 KB
+constexpr int PP_HD = 64, PP_KT = 64;  // head dim of the prompts of one length; keys of a tile
 constexpr int PP_THREADS = 12 * 32;
-constexpr uint32_t PP_CONV = 32;  // converter threads
-// operand tiles: K box j (head columns 32j..) = [64 hi rows | 64 lo rows] of
-// 128 bytes (16 KB); V key block kb = four 4 KB boxes [hi columns 0-31, hi
-// 32-63, lo 0-31, lo 32-63] of 32 keys (16 KB)
-constexpr uint32_t PP_KBOX = 2 * PP_KT * 128, PP_VBLK = 4 * 4096, PP_KVOP = 2 * PP_KVT;
-// Q hi tiles, then two K and two V operand tiles (hi and lo each)
-constexpr uint32_t PP_SMEM = 2 * PP_QTILE + 4 * PP_KVOP + 1024 + 256;
+template <int HD>
+struct PpShape
+{
+    // Head dim 128 has TMEM and shared memory for one query tile and one buffer
+    // of each operand; tile B's softmax warps then convert.
+    static constexpr int NX = HD == 128 ? 1 : 2, NB = HD == 128 ? 1 : 2;
+    static constexpr uint32_t CONV = NX == 1 ? 128 : 32;    // converter threads
+    static constexpr uint32_t QTILE = 128 * HD * 4;         // one 128-row Q tile
+    static constexpr uint32_t KVT = PP_KT * HD * 4;         // one K or V tile
+    // operand tiles: K box j (head columns 32j..) = [64 hi rows | 64 lo rows] of
+    // 128 bytes (16 KB); V key block kb = 4 KB boxes of 32 keys [hi columns 0-31,
+    // hi 32-63 .., lo 0-31 ..]
+    static constexpr uint32_t KBOX = 2 * PP_KT * 128, VLO = HD / 32 * 4096, VBLK = 2 * VLO, KVOP = 2 * KVT;
+    // Q hi tiles, then NB K and NB V operand tiles (hi and lo each)
+    static constexpr uint32_t SMEM = NX * QTILE + 2 * NB * KVOP + 1024 + 256;
+    // TMEM columns of tile x: S / P [0, 64), S's hi.lo half / P lo [64, 128), O, Q lo
+    static constexpr uint32_t TX = 256, PLO = 64, O = 128, QLO = 128 + HD;
+};
 // per operand buffer b: F copy landed, R converted, E[x] consumed by tile
 // x's MMAs (index 2x + b); per query tile x: S, P, O and the final drain
 enum PpBar { PB_QF, PB_QR, PB_KF, PB_KR = PB_KF + 2, PB_KE = PB_KR + 2, PB_VF = PB_KE + 4, PB_VR = PB_VF + 2,
              PB_VE = PB_VR + 2, PB_S0 = PB_VE + 4, PB_P0 = PB_S0 + 2, PB_O0 = PB_P0 + 2, PB_FIN = PB_O0 + 2,
              PB_N = PB_FIN + 2 };
-// TMEM columns of tile x: S / P [0, 64), S's hi.lo half / P lo [64, 128), O
-// [128, 192), Q lo [192, 256)
-constexpr uint32_t PP_TX = 256, PP_PLO = 64, PP_O = 128, PP_QLO = 192;
 
 }  // namespace
 
-template <bool SPLIT3, bool PACKED>
+template <int HD, bool SPLIT3, bool PACKED>
 __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                              const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
                                                                              PfArgs a, PackedArgs pk)
 {
     using namespace tc;
+    using Pp = PpShape<HD>;
+    constexpr int NX = Pp::NX, NB = Pp::NB;
     constexpr uint32_t IDESC_S = idesc_tf32(128, PP_KT);
     constexpr uint32_t IDESC_S2 = idesc_tf32(128, 2 * PP_KT);          // [K hi | K lo]
-    constexpr uint32_t IDESC_O = idesc_tf32(128, PP_HD) | (1u << 16);  // B (V) read MN-major
+    constexpr uint32_t IDESC_O = idesc_tf32(128, HD) | (1u << 16);     // B (V) read MN-major
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem =
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* q_s = smem;                     // Q hi of tile x at x * QTILE
-    unsigned char* k_op = smem + 2 * PP_QTILE;     // K operand buffer b at b * KVOP (PP_KBOX layout)
-    unsigned char* v_op = k_op + 2 * PP_KVOP;      // V operand buffer b at b * KVOP (PP_VBLK layout)
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_op + 2 * PP_KVOP);
+    unsigned char* q_s = smem;                    // Q hi of tile x at x * QTILE
+    unsigned char* k_op = smem + NX * Pp::QTILE;  // K operand buffer b at b * KVOP (Pp::KBOX layout)
+    unsigned char* v_op = k_op + NB * Pp::KVOP;   // V operand buffer b at b * KVOP (Pp::VBLK layout)
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_op + NB * Pp::KVOP);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PB_N);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -475,8 +466,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     uint32_t kvh = 0, hc = 0, tok0 = 0, tok1 = 0;  // PACKED: heads, tokens of tile A / B
     if constexpr (PACKED)
     {
-        PackedArgs pair = pk;  // a CTA has two tiles of pk.tpt tokens
-        pair.tpt = 2 * pk.tpt;
+        PackedArgs pair = pk;  // a CTA has NX tiles of pk.tpt tokens
+        pair.tpt = NX * pk.tpt;
         pt = packed_tile<PP_THREADS>(pair, blockIdx.x);
         if (!pt.live) return;
         kvh = h / pk.nchunk;
@@ -488,7 +479,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         nkeys0 = keys_seen(pt, pt.t0 + tok0 - 1);
         nkeys = keys_seen(pt, pt.t0 + tokens - 1);
         kv_row0 = (int)pt.k0;
-        kv_col0 = (int)(kvh * PP_HD);
+        kv_col0 = (int)(kvh * HD);
     }
     // key tiles of tile A / B
     const uint32_t nt0 = (nkeys0 + PP_KT - 1) / PP_KT;
@@ -500,8 +491,8 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         for (int i = 0; i < PB_N; ++i)
         {
             uint32_t count = 1;
-            if (i == PB_QR) count = 256;  // every softmax thread writes its Q lo row
-            if (i == PB_KR || i == PB_KR + 1 || i == PB_VR || i == PB_VR + 1) count = PP_CONV;
+            if (i == PB_QR) count = 128 * NX;  // every softmax thread writes its Q lo row
+            if (i == PB_KR || i == PB_KR + 1 || i == PB_VR || i == PB_VR + 1) count = Pp::CONV;
             if (i == PB_P0 || i == PB_P0 + 1) count = 128;
             mbar_init(&bars[i], count);
         }
@@ -520,7 +511,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp < 8)
+    if (warp < 4 * NX)
     {
         // ---------------- softmax of tile x ----------------
         const int x = warp >> 2;
@@ -539,7 +530,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             q_row = pt.q0 + token;
             q_head = kvh * pk.group + hc + head;
         }
-        const uint32_t tx = tmem + PP_TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t tx = tmem + Pp::TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
         float m = -INFINITY, l = 0.f;
         bool ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_QF], 0, abort));
@@ -547,9 +538,9 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         {
             // Q lo of this row into TMEM: row r of box j holds head columns
             // 32j + 4c.. in 16-byte chunk c ^ (r % 8)
-            const unsigned char* qrow = q_s + x * PP_QTILE + r * 128;
+            const unsigned char* qrow = q_s + x * Pp::QTILE + r * 128;
 #pragma unroll
-            for (int j = 0; j < PP_HD / 32; ++j)
+            for (int j = 0; j < HD / 32; ++j)
             {
                 uint32_t u[32];
 #pragma unroll
@@ -562,7 +553,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                     u[4 * c + 2] = __float_as_uint(lo.z);
                     u[4 * c + 3] = __float_as_uint(lo.w);
                 }
-                tmem_st32(tx + PP_QLO + 32 * j, u);
+                tmem_st32(tx + Pp::QLO + 32 * j, u);
             }
             tmem_wait_st();
         }
@@ -582,7 +573,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 if constexpr (SPLIT3)
                 {
                     uint32_t w[32];
-                    tmem_ld32_async(tx + PP_PLO + c, w);
+                    tmem_ld32_async(tx + Pp::PLO + c, w);
                     tmem_wait_ld(u);
                     tmem_wait_ld(w);
 #pragma unroll
@@ -632,14 +623,14 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 {
                     // O_x(t-1) has completed: S_x(t) was issued after it
 #pragma unroll
-                    for (int c = 0; c < PP_HD; c += 32)
+                    for (int c = 0; c < HD; c += 32)
                     {
                         float v[32];
                         uint32_t u[32];
-                        tmem_ld32(tx + PP_O + c, v);
+                        tmem_ld32(tx + Pp::O + c, v);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * corr);
-                        tmem_st32(tx + PP_O + c, u);
+                        tmem_st32(tx + Pp::O + c, u);
                     }
                 }
             }
@@ -662,7 +653,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(tf32_lo<PACKED>(s[c + i]));
-                    tmem_st32(tx + PP_PLO + c, u);
+                    tmem_st32(tx + Pp::PLO + c, u);
                 }
             }
             l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
@@ -677,12 +668,12 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             {
                 tc_fence_after();
                 const float inv = PACKED && seen == 0 ? 0.f : 1.0f / l;
-                float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * PP_HD;
+                float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
 #pragma unroll
-                for (int c = 0; c < PP_HD; c += 32)
+                for (int c = 0; c < HD; c += 32)
                 {
                     float v[32];
-                    tmem_ld32(tx + PP_O + c, v);
+                    tmem_ld32(tx + Pp::O + c, v);
                     if (live)
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
@@ -693,32 +684,33 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
         }
         if (PACKED && ok && nt == 0 && live)
         {
-            float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * PP_HD;
-            for (int i = 0; i < PP_HD; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+            float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
+            for (int i = 0; i < HD; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
-    else if (warp == 8)
+    else if (NX == 1 ? warp < 8 : warp == 8)
     {
         // ---------------- converter ----------------
-        const int ct = tid - 256;
+        constexpr int NK = 512 / Pp::CONV, NV = HD / 32 * 256 / Pp::CONV;  // float4 of a box, of a block, each
+        const int ct = tid - 128 * NX;
         for (uint32_t t = 0; t < ntiles; ++t)
         {
-            const uint32_t bf = t & 1u, ph = t >> 1;
+            const uint32_t bf = t % NB, ph = t / NB;
             // K(t): lo rows from the hi rows the copy wrote (box j = 512
             // float4 hi, then 512 lo)
             if (!mbar_wait_or(&bars[PB_KF + bf], ph, abort)) break;
             if constexpr (SPLIT3)
             {
-                // 16 loads in flight per thread before the stores
+                // loads in flight before the stores
 #pragma unroll
-                for (int c = 0; c < PP_HD / 32; ++c)
+                for (int c = 0; c < HD / 32; ++c)
                 {
-                    float4* box = reinterpret_cast<float4*>(k_op + bf * PP_KVOP + c * PP_KBOX);
-                    float4 v[16];
+                    float4* box = reinterpret_cast<float4*>(k_op + bf * Pp::KVOP + c * Pp::KBOX);
+                    float4 v[NK];
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) v[n] = box[ct + 32 * n];
+                    for (int n = 0; n < NK; ++n) v[n] = box[ct + Pp::CONV * n];
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) box[512 + ct + 32 * n] = tf32_lo4_as<PACKED>(v[n]);
+                    for (int n = 0; n < NK; ++n) box[512 + ct + Pp::CONV * n] = tf32_lo4_as<PACKED>(v[n]);
                 }
             }
             fence_async_smem();
@@ -733,30 +725,30 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
 #pragma unroll
                 for (int c = 0; c < PP_KT / 32; ++c)
                 {
-                    float4* blk = reinterpret_cast<float4*>(v_op + bf * PP_KVOP + c * PP_VBLK);
+                    float4* blk = reinterpret_cast<float4*>(v_op + bf * Pp::KVOP + c * Pp::VBLK);
                     if (valid == (uint32_t)PP_KT)
                     {
                         if constexpr (SPLIT3)
                         {
-                            float4 v[16];
+                            float4 v[NV];
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) v[n] = blk[ct + 32 * n];
+                            for (int n = 0; n < NV; ++n) v[n] = blk[ct + Pp::CONV * n];
 #pragma unroll
-                            for (int n = 0; n < 16; ++n) blk[512 + ct + 32 * n] = tf32_lo4_as<PACKED>(v[n]);
+                            for (int n = 0; n < NV; ++n) blk[Pp::VLO / 16 + ct + Pp::CONV * n] = tf32_lo4_as<PACKED>(v[n]);
                         }
                     }
                     else
                     {
-                        for (int n = 0; n < 16; ++n)
+                        for (int n = 0; n < NV; ++n)
                         {
-                            const uint32_t i = ct + 32 * n, key = c * 32 + (i % 256) / 8;
+                            const uint32_t i = ct + Pp::CONV * n, key = c * 32 + (i % 256) / 8;
                             if (key >= valid)
                             {
                                 blk[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if constexpr (SPLIT3) blk[512 + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if constexpr (SPLIT3) blk[Pp::VLO / 16 + i] = make_float4(0.f, 0.f, 0.f, 0.f);
                             }
                             else if constexpr (SPLIT3)
-                                blk[512 + i] = tf32_lo4_as<PACKED>(blk[i]);
+                                blk[Pp::VLO / 16 + i] = tf32_lo4_as<PACKED>(blk[i]);
                         }
                     }
                 }
@@ -765,7 +757,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             mbar_arrive(&bars[PB_VR + bf]);
         }
     }
-    else if (warp < 11)
+    else if (warp == 9 || warp == 10)
     {
         // ---------------- MMA issue for tile x ----------------
         const int x = __shfl_sync(FULL_MASK, warp, 0) - 9;  // the same in the warp for the compiler too
@@ -775,30 +767,30 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             auto wait = [&](int i, uint32_t ph) { return __all_sync(FULL_MASK, mbar_wait_or(&bars[i], ph, abort)) != 0; };
             // descriptors: one base each, advanced by (byte offset >> 4) in
             // the start-address field (shared addresses stay below 2^18)
-            const uint64_t dq = smem_desc(q_s + x * PP_QTILE, 0);
+            const uint64_t dq = smem_desc(q_s + x * Pp::QTILE, 0);
             const uint64_t dk = smem_desc(k_op, 0), dv = desc_mn(v_op);
-            const uint32_t ts = tmem + PP_TX * x, to = ts + PP_O;
+            const uint32_t ts = tmem + Pp::TX * x, to = ts + Pp::O;
             bool ok = wait(PB_QR, 0);
             for (uint32_t t = 0; ok && t < nt; ++t)
             {
-                const uint32_t bf = t & 1u, ph = t >> 1;
+                const uint32_t bf = t % NB, ph = t / NB;
                 // S_x(t) = Q_x K(t)^T, after O_x(t-1) has read P_x(t-1)
                 if (!(ok = wait(PB_KR + bf, ph))) break;
                 if (t > 0 && !(ok = wait(PB_O0 + x, t - 1))) break;
                 tc_fence_after();
-                const uint64_t kbase = dk + ((bf * PP_KVOP) >> 4);
+                const uint64_t kbase = dk + ((bf * Pp::KVOP) >> 4);
 #pragma unroll
-                for (int j = 0; j < PP_HD / 32; ++j)
+                for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
                     {
                         const uint64_t da = dq + ((j * (128 * 128) + kk * 32) >> 4);
-                        const uint64_t db = kbase + ((j * PP_KBOX + kk * 32) >> 4);
+                        const uint64_t db = kbase + ((j * Pp::KBOX + kk * 32) >> 4);
                         if constexpr (SPLIT3)
                         {
                             // [hi.hi | hi.lo] in one MMA, then lo.hi (Q lo from TMEM) into the first half
                             mma_tf32_elected(ts, da, db, IDESC_S2, j > 0 || kk > 0);
-                            mma_tf32_tmem_a_elected(ts, ts + PP_QLO + 32 * j + 8 * kk, db, IDESC_S, true);
+                            mma_tf32_tmem_a_elected(ts, ts + Pp::QLO + 32 * j + 8 * kk, db, IDESC_S, true);
                         }
                         else
                             mma_tf32_elected(ts, da, db, IDESC_S, j > 0 || kk > 0);
@@ -809,19 +801,19 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
                 if (!(ok = wait(PB_VR + bf, ph))) break;
                 if (!(ok = wait(PB_P0 + x, t))) break;
                 tc_fence_after();
-                const uint64_t vbase = dv + ((bf * PP_KVOP) >> 4);
+                const uint64_t vbase = dv + ((bf * Pp::KVOP) >> 4);
 #pragma unroll
                 for (int kb = 0; kb < PP_KT / 32; ++kb)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
                     {
-                        const uint64_t db = vbase + ((kb * PP_VBLK + kk * 1024) >> 4);
+                        const uint64_t db = vbase + ((kb * Pp::VBLK + kk * 1024) >> 4);
                         const uint32_t col = kb * 32 + kk * 8;
                         mma_tf32_tmem_a_elected(to, ts + col, db, IDESC_O, t > 0 || kb > 0 || kk > 0);
                         if constexpr (SPLIT3)
                         {
-                            mma_tf32_tmem_a_elected(to, ts + col, db + (8192 >> 4), IDESC_O, true);  // P hi . V lo
-                            mma_tf32_tmem_a_elected(to, ts + PP_PLO + col, db, IDESC_O, true);      // P lo . V hi
+                            mma_tf32_tmem_a_elected(to, ts + col, db + (Pp::VLO >> 4), IDESC_O, true);  // P hi . V lo
+                            mma_tf32_tmem_a_elected(to, ts + Pp::PLO + col, db, IDESC_O, true);      // P lo . V hi
                         }
                     }
                 mma_commit_elected(&bars[PB_O0 + x]);
@@ -832,43 +824,44 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             __all_sync(FULL_MASK, mbar_wait(&bars[PB_FIN + x], 0));
         }
     }
-    else
+    else if (warp == 11)
     {
         // ---------------- TMA copies ----------------
         if (lane == 0)
         {
             const int nq = has_b ? 2 : 1;
-            mbar_arrive_expect_tx(&bars[PB_QF], PACKED ? nq * (PP_HD / 32) * pk.gs * pk.tpt * 128 : nq * PP_QTILE);
+            mbar_arrive_expect_tx(&bars[PB_QF], PACKED ? nq * (HD / 32) * pk.gs * pk.tpt * 128 : nq * Pp::QTILE);
             for (int x = 0; x < nq; ++x)
-                for (int j = 0; j < PP_HD / 32; ++j)
+                for (int j = 0; j < HD / 32; ++j)
                     if constexpr (PACKED)
-                        tma_load_3d(q_s + x * PP_QTILE + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
+                        tma_load_3d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
                                     (int)(pt.q0 + pt.t0 + x * pk.tpt), &bars[PB_QF]);
                     else
-                        tma_load_2d(q_s + x * PP_QTILE + j * (128 * 128), &map_q, (int)(h * PP_HD) + 32 * j,
+                        tma_load_2d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, (int)(h * HD) + 32 * j,
                                     (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
             uint32_t issued = 0;
             for (uint32_t t = 0; t < ntiles; ++t)
             {
-                const uint32_t bf = t & 1u;
-                // K(t) into buffer t % 2 once S_A(t-2) and S_B(t-2) have read it
-                if (t >= 2 && t - 2 < nt0 && !mbar_wait_or(&bars[PB_KE + bf], (t >> 1) - 1, abort)) break;
-                if (t >= 2 && t - 2 < nt1 && !mbar_wait_or(&bars[PB_KE + 2 + bf], (t >> 1) - 1, abort)) break;
-                mbar_arrive_expect_tx(&bars[PB_KF + bf], PP_KVT);
-                for (int j = 0; j < PP_HD / 32; ++j)
-                    tma_load_2d(k_op + bf * PP_KVOP + j * PP_KBOX, &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * PP_KT),
+                const uint32_t bf = t % NB, ph = t / NB;
+                // K(t) into buffer t % NB once S_A(t-NB) and S_B(t-NB) have read it
+                const bool again = t >= NB;
+                if (again && t - NB < nt0 && !mbar_wait_or(&bars[PB_KE + bf], ph - 1, abort)) break;
+                if (again && t - NB < nt1 && !mbar_wait_or(&bars[PB_KE + 2 + bf], ph - 1, abort)) break;
+                mbar_arrive_expect_tx(&bars[PB_KF + bf], Pp::KVT);
+                for (int j = 0; j < HD / 32; ++j)
+                    tma_load_2d(k_op + bf * Pp::KVOP + j * Pp::KBOX, &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * PP_KT),
                                 &bars[PB_KF + bf]);
-                // V(t) once O_A(t-2) and O_B(t-2) have
-                if ((t >= 2 && t - 2 < nt0 && !mbar_wait_or(&bars[PB_VE + bf], (t >> 1) - 1, abort)) ||
-                    (t >= 2 && t - 2 < nt1 && !mbar_wait_or(&bars[PB_VE + 2 + bf], (t >> 1) - 1, abort)))
+                // V(t) once O_A(t-NB) and O_B(t-NB) have
+                if ((again && t - NB < nt0 && !mbar_wait_or(&bars[PB_VE + bf], ph - 1, abort)) ||
+                    (again && t - NB < nt1 && !mbar_wait_or(&bars[PB_VE + 2 + bf], ph - 1, abort)))
                 {
                     issued = 2 * t + 1;
                     break;
                 }
-                mbar_arrive_expect_tx(&bars[PB_VF + bf], PP_KVT);
+                mbar_arrive_expect_tx(&bars[PB_VF + bf], Pp::KVT);
                 for (int kb = 0; kb < PP_KT / 32; ++kb)
-                    for (int j = 0; j < PP_HD / 32; ++j)
-                        tma_load_2d(v_op + bf * PP_KVOP + kb * PP_VBLK + j * 4096, &map_v, kv_col0 + 32 * j,
+                    for (int j = 0; j < HD / 32; ++j)
+                        tma_load_2d(v_op + bf * Pp::KVOP + kb * Pp::VBLK + j * 4096, &map_v, kv_col0 + 32 * j,
                                     kv_row0 + (int)(t * PP_KT) + 32 * kb, &bars[PB_VF + bf]);
                 issued = 2 * t + 2;
             }
@@ -876,10 +869,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             // (bounded; immediate on the normal path).  Copy n < issued is
             // K(n / 2) for even n, V(n / 2) for odd n.
             mbar_wait(&bars[PB_QF], 0);
-            for (uint32_t n = issued >= 4 ? issued - 4 : 0; n < issued; ++n)
+            for (uint32_t n = issued >= 2 * NB ? issued - 2 * NB : 0; n < issued; ++n)
             {
                 const uint32_t t = n >> 1;
-                mbar_wait(&bars[(n & 1u ? PB_VF : PB_KF) + (t & 1u)], t >> 1);
+                mbar_wait(&bars[(n & 1u ? PB_VF : PB_KF) + t % NB], (t / NB) & 1u);
             }
         }
     }
@@ -901,7 +894,7 @@ int launch_tc_hd(const float* q, uint32_t ldq, const float* kc, const float* vc,
                  uint32_t B, uint32_t H, uint32_t P, float scale, cudaStream_t st)
 {
     using Sh = PfShape<HD>;
-    auto kern = prefill_attention_tc_kernel<HD, SPLIT3, false>;
+    auto kern = prefill_attention_tc_kernel<HD, SPLIT3>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Sh::SMEM, attr_devices));
     CUtensorMap mq, mk, mv;
@@ -913,7 +906,7 @@ int launch_tc_hd(const float* q, uint32_t ldq, const float* kc, const float* vc,
     FML_RC(tc::make_map(&mv, vc, (int)rows, HD, HD, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     PfArgs a{out, ldo, B, H, P, C, scale};
     dim3 grid((P + QB - 1) / QB, H, B);
-    kern<<<grid, 128, Sh::SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
+    kern<<<grid, 128, Sh::SMEM, st>>>(mq, mk, mv, a);
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
@@ -922,9 +915,10 @@ template <bool SPLIT3>
 int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, uint32_t C, float* out, uint32_t ldo,
               uint32_t B, uint32_t H, uint32_t P, float scale, cudaStream_t st)
 {
-    auto kern = prefill_attention_pp_kernel<SPLIT3, false>;
+    constexpr uint32_t SMEM = PpShape<PP_HD>::SMEM;
+    auto kern = prefill_attention_pp_kernel<PP_HD, SPLIT3, false>;
     static uint64_t attr_devices = 0;
-    FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)PP_SMEM, attr_devices));
+    FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
     CUtensorMap mq, mk, mv;
     const uint64_t rows = (uint64_t)B * H * C;
     FML_REQUIRE(rows < (1ull << 31) && (uint64_t)B * P < (1ull << 31), "prefill attention: %llu cache rows",
@@ -934,44 +928,32 @@ int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, ui
     FML_RC(tc::make_map(&mv, vc, (int)rows, PP_HD, PP_HD, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     PfArgs a{out, ldo, B, H, P, C, scale};
     dim3 grid((P + 255) / 256, H, B);
-    kern<<<grid, PP_THREADS, PP_SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
+    kern<<<grid, PP_THREADS, SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
 
-// Packed prompts: two tiles a CTA at head dim 64, else one.
+// Packed prompts.
 template <int HD, bool SPLIT3>
 int launch_packed(float* out, const float* q, const float* k, const float* v, PackedArgs p, cudaStream_t st)
 {
-    constexpr bool PP = HD == PP_HD;
-    constexpr uint32_t SMEM = PP ? PP_SMEM : PfShape<HD>::SMEM;
-    constexpr int KT = PP ? PP_KT : PfShape<HD>::KT;
+    using Pp = PpShape<HD>;
+    auto kern = prefill_attention_pp_kernel<HD, SPLIT3, true>;
+    static uint64_t attr_devices = 0;
+    FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Pp::SMEM, attr_devices));
     p.gs = p.group < 128u ? p.group : 128u;
     p.nchunk = (p.group + p.gs - 1) / p.gs;
     p.tpt = 128u / p.gs;
-    PackedArgs pair = p;
-    if (PP) pair.tpt = 2 * p.tpt;
-    const uint64_t tiles = packed_tiles_bound(pair), y = (uint64_t)p.kv_heads * p.nchunk;
+    PackedArgs cta = p;
+    cta.tpt = Pp::NX * p.tpt;
+    const uint64_t tiles = packed_tiles_bound(cta), y = (uint64_t)p.kv_heads * p.nchunk;
     FML_REQUIRE(tiles < (1ull << 31) && y <= 65535u, "fml_attention_packed: %u rows, %u heads", p.q_rows, p.heads);
     CUtensorMap mq, mk, mv;
     FML_RC(tc::make_map_heads(&mq, q, HD, p.heads, p.q_rows, p.ldq, p.gs, p.tpt));
-    FML_RC(tc::make_map(&mk, k, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldk, KT));
+    FML_RC(tc::make_map(&mk, k, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldk, PP_KT));
     FML_RC(tc::make_map(&mv, v, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldv, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     const PfArgs a{out, p.ldo, 0, 0, 0, 0, p.scale};
-    const dim3 grid((unsigned)tiles, (unsigned)y);
-    static uint64_t attr_devices = 0;
-    if constexpr (PP)
-    {
-        auto kern = prefill_attention_pp_kernel<SPLIT3, true>;
-        FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
-        kern<<<grid, PP_THREADS, SMEM, st>>>(mq, mk, mv, a, p);
-    }
-    else
-    {
-        auto kern = prefill_attention_tc_kernel<HD, SPLIT3, true>;
-        FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
-        kern<<<grid, 128, SMEM, st>>>(mq, mk, mv, a, p);
-    }
+    kern<<<dim3((unsigned)tiles, (unsigned)y), PP_THREADS, Pp::SMEM, st>>>(mq, mk, mv, a, p);
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
