@@ -404,14 +404,15 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 namespace {
 
 constexpr int PP_HD = 64, PP_KT = 64;  // head dim of the prompts of one length; keys of a tile
-constexpr int PP_THREADS = 12 * 32;
-template <int HD>
+template <int HD, bool PACKED>
 struct PpShape
 {
-    // Head dim 128 has TMEM and shared memory for one query tile and one buffer
-    // of each operand; tile B's softmax warps then convert.
-    static constexpr int NX = HD == 128 ? 1 : 2, NB = HD == 128 ? 1 : 2;
-    static constexpr uint32_t CONV = NX == 1 ? 128 : 32;    // converter threads
+    static constexpr int CTAS = PACKED && HD < 128 ? 2 : 1;  // on an SM
+    static constexpr int NX = PACKED ? 1 : 2, NB = PACKED ? 1 : 2;
+    // warps: 4 NX of softmax, then the converters, NX that issue the MMAs, one that copies
+    static constexpr int CW = !PACKED ? 1 : HD == 128 ? 4 : 2, MMA = 4 * NX + CW, TMA = MMA + NX;
+    static constexpr int THREADS = 32 * (TMA + 1);
+    static constexpr uint32_t CONV = 32 * CW;               // converter threads
     static constexpr uint32_t QTILE = 128 * HD * 4;         // one 128-row Q tile
     static constexpr uint32_t KVT = PP_KT * HD * 4;         // one K or V tile
     // operand tiles: K box j (head columns 32j..) = [64 hi rows | 64 lo rows] of
@@ -421,7 +422,7 @@ struct PpShape
     // Q hi tiles, then NB K and NB V operand tiles (hi and lo each)
     static constexpr uint32_t SMEM = NX * QTILE + 2 * NB * KVOP + 1024 + 256;
     // TMEM columns of tile x: S / P [0, 64), S's hi.lo half / P lo [64, 128), O, Q lo
-    static constexpr uint32_t TX = 256, PLO = 64, O = 128, QLO = 128 + HD;
+    static constexpr uint32_t TX = 256, PLO = 64, O = 128, QLO = 128 + HD, COLS = CTAS == 2 ? 256 : 512;
 };
 // per operand buffer b: F copy landed, R converted, E[x] consumed by tile
 // x's MMAs (index 2x + b); per query tile x: S, P, O and the final drain
@@ -432,13 +433,14 @@ enum PpBar { PB_QF, PB_QR, PB_KF, PB_KR = PB_KF + 2, PB_KE = PB_KR + 2, PB_VF = 
 }  // namespace
 
 template <int HD, bool SPLIT3, bool PACKED>
-__global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q,
+__global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACKED>::CTAS)
+    prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q,
                                                                              const __grid_constant__ CUtensorMap map_k,
                                                                              const __grid_constant__ CUtensorMap map_v,
                                                                              PfArgs a, PackedArgs pk)
 {
     using namespace tc;
-    using Pp = PpShape<HD>;
+    using Pp = PpShape<HD, PACKED>;
     constexpr int NX = Pp::NX, NB = Pp::NB;
     constexpr uint32_t IDESC_S = idesc_tf32(128, PP_KT);
     constexpr uint32_t IDESC_S2 = idesc_tf32(128, 2 * PP_KT);          // [K hi | K lo]
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     {
         PackedArgs pair = pk;  // a CTA has NX tiles of pk.tpt tokens
         pair.tpt = NX * pk.tpt;
-        pt = packed_tile<PP_THREADS>(pair, blockIdx.x);
+        pt = packed_tile<Pp::THREADS>(pair, blockIdx.x);
         if (!pt.live) return;
         kvh = h / pk.nchunk;
         hc = (h % pk.nchunk) * pk.gs;
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     if (warp == 0)
     {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(512)
+                     "r"(Pp::COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -511,6 +513,13 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // two CTAs of an SM: registers 2 x 256 x 128, a CTA's shared out as 128 x 152 for
+    // the softmax and 128 x 104
+    if constexpr (Pp::CTAS == 2)
+    {
+        if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    }
     if (warp < 4 * NX)
     {
         // ---------------- softmax of tile x ----------------
@@ -688,7 +697,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             for (int i = 0; i < HD; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
-    else if (NX == 1 ? warp < 8 : warp == 8)
+    else if (warp < Pp::MMA)
     {
         // ---------------- converter ----------------
         constexpr int NK = 512 / Pp::CONV, NV = HD / 32 * 256 / Pp::CONV;  // float4 of a box, of a block, each
@@ -757,10 +766,10 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             mbar_arrive(&bars[PB_VR + bf]);
         }
     }
-    else if (warp == 9 || warp == 10)
+    else if (warp < Pp::TMA)
     {
         // ---------------- MMA issue for tile x ----------------
-        const int x = __shfl_sync(FULL_MASK, warp, 0) - 9;  // the same in the warp for the compiler too
+        const int x = __shfl_sync(FULL_MASK, warp, 0) - Pp::MMA;  // the same in the warp for the compiler too
         const uint32_t nt = x ? nt1 : nt0;
         if (nt > 0)
         {
@@ -824,7 +833,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
             __all_sync(FULL_MASK, mbar_wait(&bars[PB_FIN + x], 0));
         }
     }
-    else if (warp == 11)
+    else
     {
         // ---------------- TMA copies ----------------
         if (lane == 0)
@@ -883,7 +892,7 @@ __global__ void __launch_bounds__(PP_THREADS, 1) prefill_attention_pp_kernel(con
     if (warp == 0)
     {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Pp::COLS) : "memory");
     }
 }
 
@@ -915,7 +924,7 @@ template <bool SPLIT3>
 int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, uint32_t C, float* out, uint32_t ldo,
               uint32_t B, uint32_t H, uint32_t P, float scale, cudaStream_t st)
 {
-    constexpr uint32_t SMEM = PpShape<PP_HD>::SMEM;
+    constexpr uint32_t SMEM = PpShape<PP_HD, false>::SMEM;
     auto kern = prefill_attention_pp_kernel<PP_HD, SPLIT3, false>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)SMEM, attr_devices));
@@ -928,7 +937,7 @@ int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, ui
     FML_RC(tc::make_map(&mv, vc, (int)rows, PP_HD, PP_HD, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     PfArgs a{out, ldo, B, H, P, C, scale};
     dim3 grid((P + 255) / 256, H, B);
-    kern<<<grid, PP_THREADS, SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
+    kern<<<grid, PpShape<PP_HD, false>::THREADS, SMEM, st>>>(mq, mk, mv, a, PackedArgs{});
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
@@ -937,7 +946,7 @@ int launch_pp(const float* q, uint32_t ldq, const float* kc, const float* vc, ui
 template <int HD, bool SPLIT3>
 int launch_packed(float* out, const float* q, const float* k, const float* v, PackedArgs p, cudaStream_t st)
 {
-    using Pp = PpShape<HD>;
+    using Pp = PpShape<HD, true>;
     auto kern = prefill_attention_pp_kernel<HD, SPLIT3, true>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Pp::SMEM, attr_devices));
@@ -953,7 +962,7 @@ int launch_packed(float* out, const float* q, const float* k, const float* v, Pa
     FML_RC(tc::make_map(&mk, k, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldk, PP_KT));
     FML_RC(tc::make_map(&mv, v, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldv, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     const PfArgs a{out, p.ldo, 0, 0, 0, 0, p.scale};
-    kern<<<dim3((unsigned)tiles, (unsigned)y), PP_THREADS, Pp::SMEM, st>>>(mq, mk, mv, a, p);
+    kern<<<dim3((unsigned)tiles, (unsigned)y), Pp::THREADS, Pp::SMEM, st>>>(mq, mk, mv, a, p);
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
