@@ -32,10 +32,17 @@ __global__ void __launch_bounds__(256) packed_attention_kernel(T* __restrict__ o
     float* Ks = Qs + PQ * HP;
     float* Vs = Ks + PK * HP;
     float* Ps = Vs + PK * HP;
-    const PackedTile p = packed_tile<256>(a, blockIdx.x);
+    __shared__ PackedTile found;
+    if (threadIdx.x < 32)
+    {
+        const PackedTile t = packed_tile(a, blockIdx.x / (a.kv_heads * a.nchunk));
+        if (threadIdx.x == 0) found = t;
+    }
+    __syncthreads();
+    const PackedTile p = found;
     if (!p.live) return;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const uint32_t kvh = blockIdx.y / a.nchunk, hc = (blockIdx.y % a.nchunk) * a.gs;
+    const uint32_t y = blockIdx.x % (a.kv_heads * a.nchunk), kvh = y / a.nchunk, hc = (y % a.nchunk) * a.gs;
     const uint32_t nh = min(a.gs, a.group - hc);  // heads of this tile
     const uint32_t nt = min(a.tpt, p.lq - p.t0);  // tokens
     // row r: token p.t0 + r / gs, head hc + r % gs
@@ -158,12 +165,9 @@ int launch_simt(void* out, const void* q, const void* k, const void* v, PackedAr
     auto kern = packed_attention_kernel<T, HD>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)simt_smem<HD>(), attr_devices));
-    a.gs = a.group < (uint32_t)PQ ? a.group : (uint32_t)PQ;
-    a.nchunk = (a.group + a.gs - 1) / a.gs;
-    a.tpt = PQ / a.gs;
-    const uint64_t tiles = packed_tiles_bound(a), y = (uint64_t)a.kv_heads * a.nchunk;
-    FML_REQUIRE(tiles < (1ull << 31) && y <= 65535u, "fml_attention_packed: %u rows, %u heads", a.q_rows, a.heads);
-    kern<<<dim3((unsigned)tiles, (unsigned)y), 256, simt_smem<HD>(), st>>>(
+    const uint64_t blocks = packed_items(&a, PQ, 1);
+    FML_REQUIRE(blocks < (1ull << 31), "fml_attention_packed: %u rows, %u heads", a.q_rows, a.heads);
+    kern<<<(unsigned)blocks, 256, simt_smem<HD>(), st>>>(
         static_cast<T*>(out), static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), a);
     FML_LAUNCH_CHECK();
     return FML_OK;

@@ -554,15 +554,13 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     {
         // ---------------- the next item ----------------
         const uint32_t ny = a.kv_heads * a.nchunk;
-        PackedArgs pair = a;  // an item has two tiles of a.tpt tokens
-        pair.tpt = 2 * a.tpt;
         uint32_t asked = 0;
         bool more = true;
         uint32_t block = blockIdx.x;
         for (uint32_t k = 0; more;)
         {
             Item it;
-            it.p = packed_tile_warp(pair, block / ny);
+            it.p = packed_tile(a, block / ny);
             // ask for the next block while this one is worked out
             if (lane == 0)
             {
@@ -574,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
                 const uint32_t y = block % ny;
                 it.kvh = y / a.nchunk;
                 it.hc = (y % a.nchunk) * a.gs;
-                const uint32_t tokens = min(pair.tpt, it.p.lq - it.p.t0);
+                const uint32_t tokens = min(a.step, it.p.lq - it.p.t0);
                 it.tok0 = min(a.tpt, tokens);
                 it.tok1 = tokens - it.tok0;
                 it.n0 = (keys_seen(it.p, it.p.t0 + it.tok0 - 1) + KH - 1) / KH;
@@ -647,12 +645,7 @@ int launch(void* out, const void* q, const void* k, const void* v, int type, Pac
     auto kern = packed_attention_tc_kernel<T, HD>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Sh::SMEM, attr_devices));
-    a.gs = a.group < 128u ? a.group : 128u;
-    a.nchunk = (a.group + a.gs - 1) / a.gs;
-    a.tpt = 128u / a.gs;
-    PackedArgs pair = a;
-    pair.tpt = 2 * a.tpt;
-    const uint64_t ctas = packed_tiles_bound(pair) * a.kv_heads * a.nchunk;
+    const uint64_t ctas = packed_items(&a, 128, 2);
     FML_REQUIRE(ctas < (1ull << 31), "fml_attention_packed: %u rows of %u heads", a.q_rows, a.heads);
     CUtensorMap mq, mk, mv;
     FML_RC(make_map_16(&mq, q, type, HD, a.heads, a.q_rows, a.ldq, Sh::COLS, a.gs, a.tpt, false));

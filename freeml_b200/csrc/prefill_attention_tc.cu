@@ -458,28 +458,30 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // heaviest query blocks (most key tiles) first
     const uint32_t qblk = gridDim.x - 1 - blockIdx.x;
-    const uint32_t q0 = qblk * 256, h = blockIdx.y, b = blockIdx.z;
+    const uint32_t q0 = qblk * 256, h = PACKED ? blockIdx.x % (pk.kv_heads * pk.nchunk) : blockIdx.y, b = blockIdx.z;
     const uint32_t P = a.P;
     bool has_b = q0 + 128 < P;
     // the keys that tile A's rows see, and any row of the CTA
     uint32_t nkeys0 = min(q0 + 128u, P), nkeys = min(q0 + 256u, P);
     int kv_row0 = (int)((b * a.H + h) * a.C), kv_col0 = 0;
     PackedTile pt{};
-    uint32_t kvh = 0, hc = 0, tok0 = 0, tok1 = 0;  // PACKED: heads, tokens of tile A / B
+    uint32_t kvh = 0, hc = 0, tokens = 0;  // PACKED: heads, tokens of the tile
     if constexpr (PACKED)
     {
-        PackedArgs pair = pk;  // a CTA has NX tiles of pk.tpt tokens
-        pair.tpt = NX * pk.tpt;
-        pt = packed_tile<Pp::THREADS>(pair, blockIdx.x);
+        __shared__ PackedTile found;
+        if (warp == 0)
+        {
+            const PackedTile t = packed_tile(pk, blockIdx.x / (pk.kv_heads * pk.nchunk));
+            if (lane == 0) found = t;
+        }
+        __syncthreads();
+        pt = found;
         if (!pt.live) return;
         kvh = h / pk.nchunk;
         hc = (h % pk.nchunk) * pk.gs;
-        const uint32_t tokens = min(pair.tpt, pt.lq - pt.t0);
-        tok0 = min(pk.tpt, tokens);
-        tok1 = tokens - tok0;
-        has_b = tok1 > 0;
-        nkeys0 = keys_seen(pt, pt.t0 + tok0 - 1);
-        nkeys = keys_seen(pt, pt.t0 + tokens - 1);
+        tokens = min(pk.tpt, pt.lq - pt.t0);
+        has_b = false;
+        nkeys0 = nkeys = keys_seen(pt, pt.t0 + tokens - 1);
         kv_row0 = (int)pt.k0;
         kv_col0 = (int)(kvh * HD);
     }
@@ -532,8 +534,8 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         if constexpr (PACKED)
         {
             const uint32_t tok = (uint32_t)r / pk.gs, head = (uint32_t)r % pk.gs;
-            live = tok < (x ? tok1 : tok0) && head < min(pk.gs, pk.group - hc);
-            const uint32_t token = pt.t0 + (x ? pk.tpt : 0u) + tok;
+            live = tok < tokens && head < min(pk.gs, pk.group - hc);
+            const uint32_t token = pt.t0 + tok;
             seen = live ? keys_seen(pt, token) : 0xffffffffu;  // rows that are no query's are left unmasked
             least = __reduce_min_sync(FULL_MASK, seen);
             q_row = pt.q0 + token;
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                 for (int j = 0; j < HD / 32; ++j)
                     if constexpr (PACKED)
                         tma_load_3d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
-                                    (int)(pt.q0 + pt.t0 + x * pk.tpt), &bars[PB_QF]);
+                                    (int)(pt.q0 + pt.t0), &bars[PB_QF]);
                     else
                         tma_load_2d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, (int)(h * HD) + 32 * j,
                                     (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
@@ -950,19 +952,14 @@ int launch_packed(float* out, const float* q, const float* k, const float* v, Pa
     auto kern = prefill_attention_pp_kernel<HD, SPLIT3, true>;
     static uint64_t attr_devices = 0;
     FML_RC(smem_limit_once(reinterpret_cast<const void*>(kern), (int)Pp::SMEM, attr_devices));
-    p.gs = p.group < 128u ? p.group : 128u;
-    p.nchunk = (p.group + p.gs - 1) / p.gs;
-    p.tpt = 128u / p.gs;
-    PackedArgs cta = p;
-    cta.tpt = Pp::NX * p.tpt;
-    const uint64_t tiles = packed_tiles_bound(cta), y = (uint64_t)p.kv_heads * p.nchunk;
-    FML_REQUIRE(tiles < (1ull << 31) && y <= 65535u, "fml_attention_packed: %u rows, %u heads", p.q_rows, p.heads);
+    const uint64_t blocks = packed_items(&p, 128, 1);
+    FML_REQUIRE(blocks < (1ull << 31), "fml_attention_packed: %u rows, %u heads", p.q_rows, p.heads);
     CUtensorMap mq, mk, mv;
     FML_RC(tc::make_map_heads(&mq, q, HD, p.heads, p.q_rows, p.ldq, p.gs, p.tpt));
     FML_RC(tc::make_map(&mk, k, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldk, PP_KT));
     FML_RC(tc::make_map(&mv, v, (int)p.k_rows, (int)(p.kv_heads * HD), (int)p.ldv, 32, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B));
     const PfArgs a{out, p.ldo, 0, 0, 0, 0, p.scale};
-    kern<<<dim3((unsigned)tiles, (unsigned)y), Pp::THREADS, Pp::SMEM, st>>>(mq, mk, mv, a, p);
+    kern<<<(unsigned)blocks, Pp::THREADS, Pp::SMEM, st>>>(mq, mk, mv, a, p);
     FML_LAUNCH_CHECK();
     return FML_OK;
 }
