@@ -388,16 +388,20 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 // overwrites the columns P_x(t-1) is read from).
 //
 // PACKED: the same over packed prompts with grouped heads (packed.cuh) at head
-// dims 32, 64 and 128: the CTA's rows are (token, query head) pairs of one
-// key/value head, each with the number of keys that it sees.  The remainders
-// are rounded to TF32 there (the product truncates them otherwise, which
-// doubles the error), and head dim 128 runs one query tile and one buffer of
-// K and V (PpShape).  Bound by the tensor pipe's three TF32 products and by the
-// softmax warps' time between them.  Measured on a B200, one causal prompt of
-// 512 tokens: 4 heads of 32 25 us, 8 of 64 32 us, 32 on 8 of 128 35 us (one
-// tile with S and P V through registers, the first kernel's way: 48, 61, 91 us;
-// CUDA cores: 43, 61, 151 us); 64 ragged prompts of 1 to 512 tokens, 8 heads of
-// 64: 48 us.
+// dims 32, 64 and 128: a CTA has ONE tile of (token, query head) rows of one
+// key/value head, each with the number of keys that it sees, one buffer of K
+// and of V, and two softmax warps to a row, half of the keys each (their maxima
+// meet in shared memory).  At head dims 32 and 64 two such CTAs share an SM, so
+// that one's start, waits and end lie under the other's work: 64 ragged prompts
+// of 8 heads of 64 take 51 us, with the two tiles above and one CTA 84 us (each
+// in the order that it likes best); head dim 128 has shared memory for one.
+// The remainders are rounded to TF32 (the product would cut them, which doubles
+// the error).  What bounds it: a step of 64 keys is a chain of S, softmax and
+// P V of about 4000 cycles, the tensor cores' share 1536 at head dim 64; two
+// CTAs overlap theirs only in part.  Measured on a B200, one causal prompt of
+// 512 tokens: 4 heads of 32 20 us, 8 of 64 25 us, 32 on 8 of 128 35 us (on the
+// CUDA cores 43, 61 and 151 us; of 1 token 6.0 against 7.4, 6.8 against 10, 8.4
+// against 15: the tensor cores take every size whose alignment they can).
 // Every wait is bounded and also returns early once any role has recorded an
 // expiry in the CTA's abort flag; the MMA thread then waits for its MMAs and
 // the copy thread for its copies (bounded) before TMEM is freed.
@@ -407,10 +411,12 @@ constexpr int PP_HD = 64, PP_KT = 64;  // head dim of the prompts of one length;
 template <int HD, bool PACKED>
 struct PpShape
 {
+    // two CTAs of an SM have 256 TMEM columns, half of the shared memory and 80 registers a thread each
     static constexpr int CTAS = PACKED && HD < 128 ? 2 : 1;  // on an SM
     static constexpr int NX = PACKED ? 1 : 2, NB = PACKED ? 1 : 2;
-    // warps: 4 NX of softmax, then the converters, NX that issue the MMAs, one that copies
-    static constexpr int CW = !PACKED ? 1 : HD == 128 ? 4 : 2, MMA = 4 * NX + CW, TMA = MMA + NX;
+    static constexpr int SPLIT = PACKED ? 2 : 1;             // softmax warps that share a row's keys
+    // warps: 4 NX SPLIT of softmax, then the converters, NX that issue the MMAs, one that copies
+    static constexpr int SM = 4 * NX * SPLIT, CW = !PACKED ? 1 : HD == 128 ? 4 : 2, MMA = SM + CW, TMA = MMA + NX;
     static constexpr int THREADS = 32 * (TMA + 1);
     static constexpr uint32_t CONV = 32 * CW;               // converter threads
     static constexpr uint32_t QTILE = 128 * HD * 4;         // one 128-row Q tile
@@ -434,10 +440,8 @@ enum PpBar { PB_QF, PB_QR, PB_KF, PB_KR = PB_KF + 2, PB_KE = PB_KR + 2, PB_VF = 
 
 template <int HD, bool SPLIT3, bool PACKED>
 __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACKED>::CTAS)
-    prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q,
-                                                                             const __grid_constant__ CUtensorMap map_k,
-                                                                             const __grid_constant__ CUtensorMap map_v,
-                                                                             PfArgs a, PackedArgs pk)
+    prefill_attention_pp_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                const __grid_constant__ CUtensorMap map_v, PfArgs a, PackedArgs pk)
 {
     using namespace tc;
     using Pp = PpShape<HD, PACKED>;
@@ -495,9 +499,9 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         for (int i = 0; i < PB_N; ++i)
         {
             uint32_t count = 1;
-            if (i == PB_QR) count = 128 * NX;  // every softmax thread writes its Q lo row
+            if (i == PB_QR) count = 32 * Pp::SM;  // every softmax thread writes its Q lo row
             if (i == PB_KR || i == PB_KR + 1 || i == PB_VR || i == PB_VR + 1) count = Pp::CONV;
-            if (i == PB_P0 || i == PB_P0 + 1) count = 128;
+            if (i == PB_P0 || i == PB_P0 + 1) count = 128 * Pp::SPLIT;
             mbar_init(&bars[i], count);
         }
         *abort = 0;
@@ -515,17 +519,15 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    // two CTAs of an SM: registers 2 x 256 x 128, a CTA's shared out as 128 x 152 for
-    // the softmax and 128 x 104
-    if constexpr (Pp::CTAS == 2)
+    if (warp < Pp::SM)
     {
-        if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    }
-    if (warp < 4 * NX)
-    {
-        // ---------------- softmax of tile x ----------------
-        const int x = warp >> 2;
+        // ---------------- softmax of tile x: keys c0 .. c0 + KS - 1 of its key tiles ----------------
+        constexpr int SPLIT = Pp::SPLIT, KS = PP_KT / SPLIT, OS = HD / SPLIT;
+        const int x = SPLIT == 1 ? warp >> 2 : 0, part = SPLIT == 1 ? 0 : warp >> 2;
+        const int c0 = part * KS, o0 = part * OS;  // its keys; the output columns that it scales and writes
+        __shared__ float row_max[SPLIT][2][128], row_sum[SPLIT][128];
+        // the other warp of the row: both come here equally often, whatever became of their waits
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory"); };
         const uint32_t nt = x ? nt1 : nt0;
         const int r = 32 * (warp & 3) + lane;                 // row within the tile
         const uint32_t row = q0 + 128u * x + (uint32_t)r;     // this thread's query row
@@ -553,6 +555,7 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j)
             {
+                if (SPLIT == 2 && (j & 1) != part) continue;
                 uint32_t u[32];
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
@@ -570,59 +573,69 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         }
         tc_fence_before();
         mbar_arrive(&bars[PB_QR]);
-        for (uint32_t t = 0; ok && t < nt; ++t)
+        for (uint32_t t = 0; SPLIT == 2 ? t < nt : ok && t < nt; ++t)
         {
-            ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_S0 + x], t, abort));
-            if (!ok) break;
-            tc_fence_after();
-            float s[PP_KT];
-#pragma unroll
-            for (int c = 0; c < PP_KT; c += 32)
+            ok = ok && __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_S0 + x], t, abort));
+            if (SPLIT == 1 && !ok) break;
+            float s[KS], mt = -INFINITY;
+            if (ok)
             {
-                uint32_t u[32];
-                tmem_ld32_async(tx + c, u);
-                if constexpr (SPLIT3)
-                {
-                    uint32_t w[32];
-                    tmem_ld32_async(tx + Pp::PLO + c, w);
-                    tmem_wait_ld(u);
-                    tmem_wait_ld(w);
+                tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]) + __uint_as_float(w[i]);
+                for (int c = 0; c < KS; c += 32)
+                {
+                    uint32_t u[32];
+                    tmem_ld32_async(tx + c0 + c, u);
+                    if constexpr (SPLIT3)
+                    {
+                        uint32_t w[32];
+                        tmem_ld32_async(tx + Pp::PLO + c0 + c, w);
+                        tmem_wait_ld(u);
+                        tmem_wait_ld(w);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]) + __uint_as_float(w[i]);
+                    }
+                    else
+                    {
+                        tmem_wait_ld(u);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]);
+                    }
+                }
+                const uint32_t k0 = t * PP_KT + c0;
+                // the mask only bites in tiles that reach past the warp's first
+                // row or past the prompt (a warp-uniform test)
+                const uint32_t row0 = row - lane;
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (PACKED ? k0 + KS <= least : k0 + KS - 1 <= row0 && k0 + KS <= P)
+                {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+                    {
+                        s[i] *= sl2;
+                        mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+                    }
                 }
                 else
                 {
-                    tmem_wait_ld(u);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]);
+                    for (int i = 0; i < KS; ++i)
+                    {
+                        const uint32_t key = k0 + i;
+                        const bool in = PACKED ? key < seen : key <= row && key < P;
+                        s[i] = in ? s[i] * sl2 : -INFINITY;  // a select: masked slots may hold NaN
+                        mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
+                    }
                 }
+                mt = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             }
-            const uint32_t k0 = t * PP_KT;
-            // the mask only bites in tiles that reach past the warp's first
-            // row or past the prompt (a warp-uniform test)
-            const uint32_t row0 = row - lane;
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (PACKED ? k0 + PP_KT <= least : k0 + PP_KT - 1 <= row0 && k0 + PP_KT <= P)
+            if constexpr (SPLIT == 2)
             {
-#pragma unroll
-                for (int i = 0; i < PP_KT; ++i)
-                {
-                    s[i] *= sl2;
-                    mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
-                }
+                row_max[part][t & 1u][r] = mt;
+                meet();
+                mt = fmaxf(mt, row_max[part ^ 1][t & 1u][r]);
+                if (!ok) continue;
             }
-            else
-            {
-#pragma unroll
-                for (int i = 0; i < PP_KT; ++i)
-                {
-                    const uint32_t key = k0 + i;
-                    const bool in = PACKED ? key < seen : key <= row && key < P;
-                    s[i] = in ? s[i] * sl2 : -INFINITY;  // a select: masked slots may hold NaN
-                    mx4[i & 3] = fmaxf(mx4[i & 3], s[i]);
-                }
-            }
-            const float mt = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             const bool need = mt > m + 8.0f;
             if (__any_sync(FULL_MASK, need))
             {
@@ -633,22 +646,25 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                 if (t > 0)
                 {
                     // O_x(t-1) has completed: S_x(t) was issued after it
+                    constexpr int OC = OS < 32 ? OS : 32;
 #pragma unroll
-                    for (int c = 0; c < HD; c += 32)
+                    for (int c = 0; c < OS; c += OC)
                     {
-                        float v[32];
-                        uint32_t u[32];
-                        tmem_ld32(tx + Pp::O + c, v);
+                        float v[OC];
+                        uint32_t u[OC];
+                        if constexpr (OC == 32) tmem_ld32(tx + Pp::O + o0 + c, v);
+                        else tmem_ld16(tx + Pp::O + o0 + c, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * corr);
-                        tmem_st32(tx + Pp::O + c, u);
+                        for (int i = 0; i < OC; ++i) u[i] = __float_as_uint(v[i] * corr);
+                        if constexpr (OC == 32) tmem_st32(tx + Pp::O + o0 + c, u);
+                        else tmem_st16(tx + Pp::O + o0 + c, u);
                     }
                 }
             }
             float ls[4] = {0.f, 0.f, 0.f, 0.f};
             const float base = PACKED && m == -INFINITY ? 0.f : m;  // a packed row may see no key
 #pragma unroll
-            for (int c = 0; c < PP_KT; c += 32)
+            for (int c = 0; c < KS; c += 32)
             {
                 uint32_t u[32];
 #pragma unroll
@@ -659,18 +675,24 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                     s[c + i] = p;
                     u[i] = __float_as_uint(p);
                 }
-                tmem_st32(tx + c, u);  // P over S's columns (the MMA reads its TF32 part)
+                tmem_st32(tx + c0 + c, u);  // P over S's columns (the MMA reads its TF32 part)
                 if constexpr (SPLIT3)
                 {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(tf32_lo<PACKED>(s[c + i]));
-                    tmem_st32(tx + Pp::PLO + c, u);
+                    tmem_st32(tx + Pp::PLO + c0 + c, u);
                 }
             }
             l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&bars[PB_P0 + x]);
+        }
+        if constexpr (SPLIT == 2)
+        {
+            row_sum[part][r] = l;
+            meet();
+            l = row_sum[0][r] + row_sum[1][r];
         }
         if (ok && nt > 0)
         {
@@ -679,15 +701,17 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             {
                 tc_fence_after();
                 const float inv = PACKED && seen == 0 ? 0.f : 1.0f / l;
-                float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
+                float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD + o0;
+                constexpr int OC = OS < 32 ? OS : 32;
 #pragma unroll
-                for (int c = 0; c < HD; c += 32)
+                for (int c = 0; c < OS; c += OC)
                 {
-                    float v[32];
-                    tmem_ld32(tx + Pp::O + c, v);
+                    float v[OC];
+                    if constexpr (OC == 32) tmem_ld32(tx + Pp::O + o0 + c, v);
+                    else tmem_ld16(tx + Pp::O + o0 + c, v);
                     if (live)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
+                        for (int i = 0; i < OC; i += 4)
                             *reinterpret_cast<float4*>(dst + c + i) =
                                 make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
                 }
@@ -696,14 +720,14 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         if (PACKED && ok && nt == 0 && live)
         {
             float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD;
-            for (int i = 0; i < HD; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = o0; i < o0 + OS; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
     else if (warp < Pp::MMA)
     {
         // ---------------- converter ----------------
         constexpr int NK = 512 / Pp::CONV, NV = HD / 32 * 256 / Pp::CONV;  // float4 of a box, of a block, each
-        const int ct = tid - 128 * NX;
+        const int ct = tid - 32 * Pp::SM;
         for (uint32_t t = 0; t < ntiles; ++t)
         {
             const uint32_t bf = t % NB, ph = t / NB;

@@ -106,20 +106,8 @@ __device__ __forceinline__ void mma_tf32(uint32_t tmem_d, uint64_t da, uint64_t 
         : "memory");
 }
 
-// D (TMEM) (+)= A . B^T with A read from TMEM (lane = row, one tf32 per
-// 32-bit column along K) and B from shared memory; one K = 8 step.
-__device__ __forceinline__ void mma_tf32_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
-                                                bool accumulate)
-{
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(db), "r"(idesc), "r"((uint32_t)accumulate)
-        : "memory");
-}
-
-// The same three from a whole warp, of which the hardware elects one lane (the
+// The product (also with A read from TMEM: lane = row, one tf32 per 32-bit
+// column along K) and its commit from a whole warp, of which the hardware elects one lane (the
 // same one each time): operands are then the same in the warp for the compiler
 // too.  From a branch of one thread a product takes 80 to 130 cycles to issue,
 // more than a small one takes to run; so, 15 to 25.
