@@ -390,18 +390,22 @@ __global__ void __launch_bounds__(128, 1) prefill_attention_tc_kernel(const __gr
 // PACKED: the same over packed prompts with grouped heads (packed.cuh) at head
 // dims 32, 64 and 128: a CTA has ONE tile of (token, query head) rows of one
 // key/value head, each with the number of keys that it sees, one buffer of K
-// and of V, and two softmax warps to a row, half of the keys each (their maxima
-// meet in shared memory).  At head dims 32 and 64 two such CTAs share an SM, so
-// that one's start, waits and end lie under the other's work: 64 ragged prompts
-// of 8 heads of 64 take 51 us, with the two tiles above and one CTA 84 us (each
-// in the order that it likes best); head dim 128 has shared memory for one.
-// The remainders are rounded to TF32 (the product would cut them, which doubles
-// the error).  What bounds it: a step of 64 keys is a chain of S, softmax and
-// P V of about 4000 cycles, the tensor cores' share 1536 at head dim 64; two
-// CTAs overlap theirs only in part.  Measured on a B200, one causal prompt of
-// 512 tokens: 4 heads of 32 20 us, 8 of 64 25 us, 32 on 8 of 128 35 us (on the
-// CUDA cores 43, 61 and 151 us; of 1 token 6.0 against 7.4, 6.8 against 10, 8.4
-// against 15: the tensor cores take every size whose alignment they can).
+// and of V, two softmax warps to a row, half of the keys each (their maxima
+// meet in shared memory), and converters that also start the copies.  At head
+// dims 32 and 64 two such CTAs share an SM, so that one's start, waits and end
+// lie under the other's work: 64 ragged prompts of 8 heads of 64 take 54 us,
+// with the two tiles above and one CTA 84 us.  Head dim 128 has shared memory
+// for one.
+// Precision: the tensor cores cut their running sums, so a key tile's P V is a
+// sum of its own, added to the row's in registers (kept in TMEM over all keys
+// it is 1.6e-5 off after 3300 keys, so 5e-7, and 9 % faster); the small terms go
+// into sums of their own (S) or first (P V); remainders are rounded to TF32.
+// What bounds it: a step of 64 keys is a chain of S, softmax and P V of about
+// 4500 cycles, the tensor cores' share 1536 at head dim 64; two CTAs overlap
+// theirs only in part.  Measured on a B200, one causal prompt of 512 tokens: 4
+// heads of 32 21 us, 8 of 64 26 us, 32 on 8 of 128 37 us (on the CUDA cores 43,
+// 61 and 151 us; of 1 token 6.1 against 7.4, 7.3 against 10, 8.9 against 15: the
+// tensor cores take every call whose alignment and scale they can).
 // Every wait is bounded and also returns early once any role has recorded an
 // expiry in the CTA's abort flag; the MMA thread then waits for its MMAs and
 // the copy thread for its copies (bounded) before TMEM is freed.
@@ -415,9 +419,10 @@ struct PpShape
     static constexpr int CTAS = PACKED && HD < 128 ? 2 : 1;  // on an SM
     static constexpr int NX = PACKED ? 1 : 2, NB = PACKED ? 1 : 2;
     static constexpr int SPLIT = PACKED ? 2 : 1;             // softmax warps that share a row's keys
-    // warps: 4 NX SPLIT of softmax, then the converters, NX that issue the MMAs, one that copies
-    static constexpr int SM = 4 * NX * SPLIT, CW = !PACKED ? 1 : HD == 128 ? 4 : 2, MMA = SM + CW, TMA = MMA + NX;
-    static constexpr int THREADS = 32 * (TMA + 1);
+    // warps: 4 NX SPLIT of softmax, then the converters (PACKED: their first lane copies too), NX that
+    // issue the MMAs, and without PACKED one that copies
+    static constexpr int SM = 4 * NX * SPLIT, CW = !PACKED || HD == 32 ? 1 : HD == 64 ? 2 : 4, MMA = SM + CW, TMA = MMA + NX;
+    static constexpr int THREADS = 32 * (TMA + !PACKED);
     static constexpr uint32_t CONV = 32 * CW;               // converter threads
     static constexpr uint32_t QTILE = 128 * HD * 4;         // one 128-row Q tile
     static constexpr uint32_t KVT = PP_KT * HD * 4;         // one K or V tile
@@ -546,6 +551,21 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         const uint32_t tx = tmem + Pp::TX * x + ((uint32_t)(32 * (warp & 3)) << 16);
         const float sl2 = a.scale * 1.4426950408889634f;  // scores in log2 units
         float m = -INFINITY, l = 0.f;
+        // PACKED: the key tiles' P V, added here: the tensor cores cut their running sums, and the
+        // error would grow with the keys
+        float acc[PACKED ? OS : 1];
+#pragma unroll
+        for (int i = 0; i < (PACKED ? OS : 1); ++i) acc[i] = 0.f;
+        auto add_tile = [&] {
+#pragma unroll
+            for (int c = 0; c < OS; c += 16)
+            {
+                float v[16];
+                tmem_ld16(tx + Pp::O + o0 + c, v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[PACKED ? c + i : 0] += v[i];
+            }
+        };
         bool ok = __all_sync(FULL_MASK, mbar_wait_or(&bars[PB_QF], 0, abort));
         if (ok && SPLIT3)
         {
@@ -581,6 +601,23 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             if (ok)
             {
                 tc_fence_after();
+                // O_x(t-1) has completed: S_x(t) was issued after it
+                if (PACKED && t > 0) add_tile();
+                if constexpr (PACKED)
+                {
+                    static_assert(KS == 32, "");
+                    tmem_ld32(tx + c0, s);
+                    if constexpr (SPLIT3)
+#pragma unroll
+                        for (int c = 0; c < KS; c += 16)
+                        {
+                            float w[16];
+                            tmem_ld16(tx + Pp::PLO + c0 + c, w);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) s[c + i] += w[i];
+                        }
+                }
+                else
 #pragma unroll
                 for (int c = 0; c < KS; c += 32)
                 {
@@ -640,24 +677,26 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             if (__any_sync(FULL_MASK, need))
             {
                 const float mn = need ? mt : m;
-                const float corr = ex2_approx(m - mn);  // 0 on the first tile (m = -inf)
+                const float corr = need ? ex2_approx(m - mn) : 1.f;  // 0 on the first tile (m = -inf)
                 l *= corr;
                 m = mn;
-                if (t > 0)
+                if constexpr (PACKED)
+                {
+#pragma unroll
+                    for (int i = 0; i < OS; ++i) acc[i] *= corr;
+                }
+                else if (t > 0)
                 {
                     // O_x(t-1) has completed: S_x(t) was issued after it
-                    constexpr int OC = OS < 32 ? OS : 32;
 #pragma unroll
-                    for (int c = 0; c < OS; c += OC)
+                    for (int c = 0; c < HD; c += 32)
                     {
-                        float v[OC];
-                        uint32_t u[OC];
-                        if constexpr (OC == 32) tmem_ld32(tx + Pp::O + o0 + c, v);
-                        else tmem_ld16(tx + Pp::O + o0 + c, v);
+                        float v[32];
+                        uint32_t u[32];
+                        tmem_ld32(tx + Pp::O + c, v);
 #pragma unroll
-                        for (int i = 0; i < OC; ++i) u[i] = __float_as_uint(v[i] * corr);
-                        if constexpr (OC == 32) tmem_st32(tx + Pp::O + o0 + c, u);
-                        else tmem_st16(tx + Pp::O + o0 + c, u);
+                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(v[i] * corr);
+                        tmem_st32(tx + Pp::O + c, u);
                     }
                 }
             }
@@ -676,7 +715,16 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                     u[i] = __float_as_uint(p);
                 }
                 tmem_st32(tx + c0 + c, u);  // P over S's columns (the MMA reads its TF32 part)
-                if constexpr (SPLIT3)
+                if constexpr (SPLIT3 && PACKED)
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16)
+                    {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(tf32_lo<PACKED>(s[c + h + i]));
+                        tmem_st16(tx + Pp::PLO + c0 + c + h, w);
+                    }
+                else if constexpr (SPLIT3)
                 {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(tf32_lo<PACKED>(s[c + i]));
@@ -700,20 +748,31 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             if (ok)
             {
                 tc_fence_after();
-                const float inv = PACKED && seen == 0 ? 0.f : 1.0f / l;
+                const float inv = 1.0f / l;
                 float* dst = a.out + (uint64_t)q_row * a.ldo + (uint64_t)q_head * HD + o0;
-                constexpr int OC = OS < 32 ? OS : 32;
-#pragma unroll
-                for (int c = 0; c < OS; c += OC)
+                if constexpr (PACKED)
                 {
-                    float v[OC];
-                    if constexpr (OC == 32) tmem_ld32(tx + Pp::O + o0 + c, v);
-                    else tmem_ld16(tx + Pp::O + o0 + c, v);
+                    add_tile();
+#pragma unroll
+                    for (int i = 0; i < OS; ++i) acc[i] = seen == 0 ? 0.f : acc[i] * inv;
                     if (live)
 #pragma unroll
-                        for (int i = 0; i < OC; i += 4)
-                            *reinterpret_cast<float4*>(dst + c + i) =
-                                make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                        for (int i = 0; i < OS; i += 4)
+                            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                }
+                else
+                {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32)
+                    {
+                        float v[32];
+                        tmem_ld32(tx + Pp::O + c, v);
+                        if (live)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *reinterpret_cast<float4*>(dst + c + i) =
+                                    make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                    }
                 }
             }
         }
@@ -728,12 +787,8 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         // ---------------- converter ----------------
         constexpr int NK = 512 / Pp::CONV, NV = HD / 32 * 256 / Pp::CONV;  // float4 of a box, of a block, each
         const int ct = tid - 32 * Pp::SM;
-        for (uint32_t t = 0; t < ntiles; ++t)
-        {
-            const uint32_t bf = t % NB, ph = t / NB;
-            // K(t): lo rows from the hi rows the copy wrote (box j = 512
-            // float4 hi, then 512 lo)
-            if (!mbar_wait_or(&bars[PB_KF + bf], ph, abort)) break;
+        // K: lo rows from the hi rows the copy wrote (box j = 512 float4 hi, then 512 lo)
+        auto convert_k = [&](uint32_t bf) {
             if constexpr (SPLIT3)
             {
                 // loads in flight before the stores
@@ -750,47 +805,109 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             }
             fence_async_smem();
             mbar_arrive(&bars[PB_KR + bf]);
-            // V(t): key block kb = hi boxes (256 float4 each) then lo boxes;
-            // rows at or past `nkeys` are zeroed (the cache there may hold
-            // anything, and 0 * NaN is NaN)
-            if (!mbar_wait_or(&bars[PB_VF + bf], ph, abort)) break;
+        };
+        // V(t): key block kb = hi boxes (256 float4 each) then lo boxes; rows at or
+        // past `nkeys` are zeroed (the cache there may hold anything, and 0 * NaN is NaN)
+        auto convert_v = [&](uint32_t bf, uint32_t t) {
+            const uint32_t k0 = t * PP_KT;
+            const uint32_t valid = nkeys - k0 < (uint32_t)PP_KT ? nkeys - k0 : (uint32_t)PP_KT;
+#pragma unroll
+            for (int c = 0; c < PP_KT / 32; ++c)
             {
-                const uint32_t k0 = t * PP_KT;
-                const uint32_t valid = nkeys - k0 < (uint32_t)PP_KT ? nkeys - k0 : (uint32_t)PP_KT;
-#pragma unroll
-                for (int c = 0; c < PP_KT / 32; ++c)
+                float4* blk = reinterpret_cast<float4*>(v_op + bf * Pp::KVOP + c * Pp::VBLK);
+                if (valid == (uint32_t)PP_KT)
                 {
-                    float4* blk = reinterpret_cast<float4*>(v_op + bf * Pp::KVOP + c * Pp::VBLK);
-                    if (valid == (uint32_t)PP_KT)
+                    if constexpr (SPLIT3)
                     {
-                        if constexpr (SPLIT3)
-                        {
-                            float4 v[NV];
+                        float4 v[NV];
 #pragma unroll
-                            for (int n = 0; n < NV; ++n) v[n] = blk[ct + Pp::CONV * n];
+                        for (int n = 0; n < NV; ++n) v[n] = blk[ct + Pp::CONV * n];
 #pragma unroll
-                            for (int n = 0; n < NV; ++n) blk[Pp::VLO / 16 + ct + Pp::CONV * n] = tf32_lo4_as<PACKED>(v[n]);
-                        }
+                        for (int n = 0; n < NV; ++n) blk[Pp::VLO / 16 + ct + Pp::CONV * n] = tf32_lo4_as<PACKED>(v[n]);
                     }
-                    else
+                }
+                else
+                {
+                    for (int n = 0; n < NV; ++n)
                     {
-                        for (int n = 0; n < NV; ++n)
+                        const uint32_t i = ct + Pp::CONV * n, key = c * 32 + (i % 256) / 8;
+                        if (key >= valid)
                         {
-                            const uint32_t i = ct + Pp::CONV * n, key = c * 32 + (i % 256) / 8;
-                            if (key >= valid)
-                            {
-                                blk[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if constexpr (SPLIT3) blk[Pp::VLO / 16 + i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            }
-                            else if constexpr (SPLIT3)
-                                blk[Pp::VLO / 16 + i] = tf32_lo4_as<PACKED>(blk[i]);
+                            blk[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if constexpr (SPLIT3) blk[Pp::VLO / 16 + i] = make_float4(0.f, 0.f, 0.f, 0.f);
                         }
+                        else if constexpr (SPLIT3)
+                            blk[Pp::VLO / 16 + i] = tf32_lo4_as<PACKED>(blk[i]);
                     }
                 }
             }
             fence_async_smem();
             mbar_arrive(&bars[PB_VR + bf]);
+        };
+        if constexpr (PACKED)
+        {
+            // one buffer of each: K(t + 1) is copied and converted while the softmax of
+            // tile t runs, V(t + 1) while that of tile t + 1 does (both copies before both
+            // conversions was slower: the first conversion then waits for S)
+            static_assert(NB == 1, "");
+            uint32_t nk = 0, nv = 0;  // copies of each that the first thread has started
+            auto copy_k = [&](uint32_t t) {
+                mbar_arrive_expect_tx(&bars[PB_KF], Pp::KVT);
+                for (int j = 0; j < HD / 32; ++j)
+                    tma_load_2d(k_op + j * Pp::KBOX, &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * PP_KT), &bars[PB_KF]);
+                ++nk;
+            };
+            auto copy_v = [&](uint32_t t) {
+                mbar_arrive_expect_tx(&bars[PB_VF], Pp::KVT);
+                for (int kb = 0; kb < PP_KT / 32; ++kb)
+                    for (int j = 0; j < HD / 32; ++j)
+                        tma_load_2d(v_op + kb * Pp::VBLK + j * 4096, &map_v, kv_col0 + 32 * j,
+                                    kv_row0 + (int)(t * PP_KT) + 32 * kb, &bars[PB_VF]);
+                ++nv;
+            };
+            if (ct == 0)
+            {
+                mbar_arrive_expect_tx(&bars[PB_QF], HD / 32 * pk.gs * pk.tpt * 128);
+                for (int j = 0; j < HD / 32; ++j)
+                    tma_load_3d(q_s + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
+                                (int)(pt.q0 + pt.t0), &bars[PB_QF]);
+                if (nt0 > 0) copy_k(0), copy_v(0);
+            }
+            for (uint32_t t = 0; t < nt0; ++t)
+            {
+                if (ct == 0 && t > 0)
+                {
+                    if (!mbar_wait_or(&bars[PB_KE], t - 1, abort)) break;
+                    copy_k(t);
+                }
+                if (!mbar_wait_or(&bars[PB_KF], t, abort)) break;
+                convert_k(0);
+                if (ct == 0 && t > 0)
+                {
+                    if (!mbar_wait_or(&bars[PB_VE], t - 1, abort)) break;
+                    copy_v(t);
+                }
+                if (!mbar_wait_or(&bars[PB_VF], t, abort)) break;
+                convert_v(0, t);
+            }
+            if (ct == 0)
+            {
+                // the copies that this thread started land before the CTA exits (bounded; immediate
+                // on the normal path)
+                mbar_wait(&bars[PB_QF], 0);
+                if (nk) mbar_wait(&bars[PB_KF], (nk - 1) & 1u);
+                if (nv) mbar_wait(&bars[PB_VF], (nv - 1) & 1u);
+            }
         }
+        else
+            for (uint32_t t = 0; t < ntiles; ++t)
+            {
+                const uint32_t bf = t % NB, ph = t / NB;
+                if (!mbar_wait_or(&bars[PB_KF + bf], ph, abort)) break;
+                convert_k(bf);
+                if (!mbar_wait_or(&bars[PB_VF + bf], ph, abort)) break;
+                convert_v(bf, t);
+            }
     }
     else if (warp < Pp::TMA)
     {
@@ -825,7 +942,9 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                         {
                             // [hi.hi | hi.lo] in one MMA, then lo.hi (Q lo from TMEM) into the first half
                             mma_tf32_elected(ts, da, db, IDESC_S2, j > 0 || kk > 0);
-                            mma_tf32_tmem_a_elected(ts, ts + Pp::QLO + 32 * j + 8 * kk, db, IDESC_S, true);
+                            // (PACKED: into the second, which keeps cuts of its sum off the large one)
+                            mma_tf32_tmem_a_elected(ts + (PACKED ? Pp::PLO : 0u), ts + Pp::QLO + 32 * j + 8 * kk, db,
+                                                    IDESC_S, true);
                         }
                         else
                             mma_tf32_elected(ts, da, db, IDESC_S, j > 0 || kk > 0);
@@ -837,20 +956,26 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                 if (!(ok = wait(PB_P0 + x, t))) break;
                 tc_fence_after();
                 const uint64_t vbase = dv + ((bf * Pp::KVOP) >> 4);
+                // PACKED: the small terms of all keys first, so that fewer sums of full size are cut
 #pragma unroll
-                for (int kb = 0; kb < PP_KT / 32; ++kb)
+                for (int part = 0; part < (PACKED && SPLIT3 ? 2 : 1); ++part)
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                    {
-                        const uint64_t db = vbase + ((kb * Pp::VBLK + kk * 1024) >> 4);
-                        const uint32_t col = kb * 32 + kk * 8;
-                        mma_tf32_tmem_a_elected(to, ts + col, db, IDESC_O, t > 0 || kb > 0 || kk > 0);
-                        if constexpr (SPLIT3)
+                    for (int kb = 0; kb < PP_KT / 32; ++kb)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
                         {
-                            mma_tf32_tmem_a_elected(to, ts + col, db + (Pp::VLO >> 4), IDESC_O, true);  // P hi . V lo
-                            mma_tf32_tmem_a_elected(to, ts + Pp::PLO + col, db, IDESC_O, true);      // P lo . V hi
+                            const uint64_t db = vbase + ((kb * Pp::VBLK + kk * 1024) >> 4);
+                            const uint32_t col = kb * 32 + kk * 8;
+                            const bool more = (!PACKED && t > 0) || kb > 0 || kk > 0;
+                            if (!PACKED || !SPLIT3 || part == 1)
+                                mma_tf32_tmem_a_elected(to, ts + col, db, IDESC_O, more || part == 1);
+                            if (SPLIT3 && part == 0)
+                            {
+                                mma_tf32_tmem_a_elected(to, ts + col, db + (Pp::VLO >> 4), IDESC_O,
+                                                        more || !PACKED);                             // P hi . V lo
+                                mma_tf32_tmem_a_elected(to, ts + Pp::PLO + col, db, IDESC_O, true);  // P lo . V hi
+                            }
                         }
-                    }
                 mma_commit_elected(&bars[PB_O0 + x]);
                 mma_commit_elected(&bars[PB_VE + 2 * x + bf]);
             }
@@ -859,21 +984,17 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
             __all_sync(FULL_MASK, mbar_wait(&bars[PB_FIN + x], 0));
         }
     }
-    else
+    else if constexpr (!PACKED)
     {
         // ---------------- TMA copies ----------------
         if (lane == 0)
         {
             const int nq = has_b ? 2 : 1;
-            mbar_arrive_expect_tx(&bars[PB_QF], PACKED ? nq * (HD / 32) * pk.gs * pk.tpt * 128 : nq * Pp::QTILE);
+            mbar_arrive_expect_tx(&bars[PB_QF], nq * Pp::QTILE);
             for (int x = 0; x < nq; ++x)
                 for (int j = 0; j < HD / 32; ++j)
-                    if constexpr (PACKED)
-                        tma_load_3d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, 32 * j, (int)(kvh * pk.group + hc),
-                                    (int)(pt.q0 + pt.t0), &bars[PB_QF]);
-                    else
-                        tma_load_2d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, (int)(h * HD) + 32 * j,
-                                    (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
+                    tma_load_2d(q_s + x * Pp::QTILE + j * (128 * 128), &map_q, (int)(h * HD) + 32 * j,
+                                (int)(b * P + q0 + 128 * x), &bars[PB_QF]);
             uint32_t issued = 0;
             for (uint32_t t = 0; t < ntiles; ++t)
             {
@@ -884,7 +1005,7 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                 if (again && t - NB < nt1 && !mbar_wait_or(&bars[PB_KE + 2 + bf], ph - 1, abort)) break;
                 mbar_arrive_expect_tx(&bars[PB_KF + bf], Pp::KVT);
                 for (int j = 0; j < HD / 32; ++j)
-                    tma_load_2d(k_op + bf * Pp::KVOP + j * Pp::KBOX, &map_k, kv_col0 + 32 * j, kv_row0 + (int)(t * PP_KT),
+                    tma_load_2d(k_op + bf * Pp::KVOP + j * Pp::KBOX, &map_k, 32 * j, kv_row0 + (int)(t * PP_KT),
                                 &bars[PB_KF + bf]);
                 // V(t) once O_A(t-NB) and O_B(t-NB) have
                 if ((again && t - NB < nt0 && !mbar_wait_or(&bars[PB_VE + bf], ph - 1, abort)) ||
@@ -896,7 +1017,7 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                 mbar_arrive_expect_tx(&bars[PB_VF + bf], Pp::KVT);
                 for (int kb = 0; kb < PP_KT / 32; ++kb)
                     for (int j = 0; j < HD / 32; ++j)
-                        tma_load_2d(v_op + bf * Pp::KVOP + kb * Pp::VBLK + j * 4096, &map_v, kv_col0 + 32 * j,
+                        tma_load_2d(v_op + bf * Pp::KVOP + kb * Pp::VBLK + j * 4096, &map_v, 32 * j,
                                     kv_row0 + (int)(t * PP_KT) + 32 * kb, &bars[PB_VF + bf]);
                 issued = 2 * t + 2;
             }
