@@ -14,9 +14,10 @@
 // taken against a reference exponent that keeps p and p times the scale there;
 // p enters the output and its sum alike, so that the reference cancels.
 //   fp32: q and p go in as two halves each, hi and the remainder lo (22 bits);
-//   codes are made normal halves about their middle, code - 8, or the sums
-//   over codes would be large numbers that the minima's sums take away again
-//   (1600 keys: 2e-5 off, centred 4e-7).
+//   codes are made normal halves about their middle (code - 8 for keys, - 7.5
+//   for values), or the sums over codes would be large numbers that the minima's
+//   sums take away again (64 sequences of up to 1600 keys: 2e-5 off; centred,
+//   9e-7, the formula in plain fp32 4e-7).
 //   16-bit types: q is a half exactly; a code needs one AND to be an operand,
 //   because bits 0..3 (4..7) of a half ARE the number code * 2^-24 (2^-20).
 //   Products of such small halves are exact to about 2^-20 only, well below
@@ -147,6 +148,13 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w)
         return half2_bits(
             __hfma2(bits_half2((w & 0x00f000f0u) | 0x64006400u), bits_half2(0x2c002c00u), bits_half2(0xd480d480u)));
     return w & 0x00f000f0u;
+}
+
+// Codes 4..7 of a word's halves less 7.5, their middle.
+__device__ __forceinline__ uint32_t codes_middle(uint32_t w)
+{
+    return half2_bits(
+        __hfma2(bits_half2((w & 0x00f000f0u) | 0x64006400u), bits_half2(0x2c002c00u), bits_half2(0xd478d478u)));
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src)
@@ -372,7 +380,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     float ref[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f}, edge[2] = {-INFINITY, -INFINITY};
     float2 l = make_float2(0.f, 0.f);
     float acc[NG][2][4];  // columns 32 g + 4 n + 2 i (+ 1: the upper two) of both heads
-    float2 u2[NG];        // sum p minimum (FULL: minimum + 8 scale) over this thread's keys
+    float2 u2[NG];        // sum p minimum (FULL: minimum + 7.5 scale) over this thread's keys
     constexpr int CAP = 30;
     int span = CAP + 100;  // a fresh maximum's p is 2^span, and no p passes 2^(span + 4); not chosen yet
     uint32_t limit = 0;    // bits of a half that the values' scales stay below
@@ -538,9 +546,17 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 const uint32_t sel = (g & 1) ? 0x7632 : 0x5410;
                 const uint32_t z0 = __byte_perm(vw[0][g / 2], vw[1][g / 2], sel);
                 const uint32_t z1 = __byte_perm(vw[2][g / 2], vw[3][g / 2], sel);
+                // fp32: about 7.5, since what the codes' mean is off their middle stays in the sums over
+                // the keys until u2 takes it away again (two shifts more than about 8)
                 const uint32_t r0 = z0 >> 8, r1 = z1 >> 8;
-                const uint32_t a0[4] = {codes_low<FULL>(z0), codes_high<FULL>(z0), codes_low<FULL>(z1), codes_high<FULL>(z1)};
-                const uint32_t a1[4] = {codes_low<FULL>(r0), codes_high<FULL>(r0), codes_low<FULL>(r1), codes_high<FULL>(r1)};
+                const uint32_t a0[4] = {FULL ? codes_middle(z0 << 4) : codes_low<FULL>(z0),
+                                        FULL ? codes_middle(z0) : codes_high<FULL>(z0),
+                                        FULL ? codes_middle(z1 << 4) : codes_low<FULL>(z1),
+                                        FULL ? codes_middle(z1) : codes_high<FULL>(z1)};
+                const uint32_t a1[4] = {FULL ? codes_middle(z0 >> 4) : codes_low<FULL>(r0),
+                                        FULL ? codes_middle(r0) : codes_high<FULL>(r0),
+                                        FULL ? codes_middle(z1 >> 4) : codes_low<FULL>(r1),
+                                        FULL ? codes_middle(r1) : codes_high<FULL>(r1)};
                 uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -549,7 +565,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     split2(mul2(p[k], make_float2(v.x, v.x)), &hi[k], &lo[k]);
                     hi[k] = transpose8(hi[k]);
                     lo[k] = transpose8(lo[k]);
-                    const float mid = FULL ? fmaf(8.f, v.x, v.y) : v.y;
+                    const float mid = FULL ? fmaf(7.5f, v.x, v.y) : v.y;
                     u2[g] = fma2(p[k], make_float2(mid, mid), u2[g]);
                 }
                 if constexpr (FULL)
