@@ -30,7 +30,10 @@
 // own tiles (2560 bytes: 16, 32 or 64 keys) through a ring of cp.async stages,
 // masked keys filled with zeros, and keeps its own running maximum, sum and
 // output in registers.  Segments of a split sequence leave partial results,
-// which a second kernel joins.
+// which a second kernel joins.  About 350 instructions per 16 keys keep 62 % (fp32)
+// and 55 % (16 bit) of the issue slots busy: 64 sequences of 1600 keys, 16 heads of
+// 64, fp32, take 65 us on a B200 (2.0 TB/s); 8 of up to 65537, 32 on 8 heads of 128,
+// bf16, 81 us (3.4 TB/s).
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -45,7 +48,7 @@ constexpr int STAGES = 4;   // tiles in flight per warp
 constexpr int TILE = 2560;  // bytes of a tile
 constexpr uint32_t MIN_SEGMENT = 256;  // keys
 // CTAs an SM holds: head dim 128 needs the registers of 3 (8 long sequences of
-// grouped heads: 104 us against 113 at 4 with 128 registers a thread)
+// grouped heads: 80 us against 92 at 4 with 128 registers a thread)
 constexpr int ctas_per_sm(int head_dim) { return head_dim == 128 ? 3 : 4; }
 
 template <typename T>

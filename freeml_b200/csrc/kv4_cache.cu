@@ -5,12 +5,16 @@
 // four neighbouring threads a group of 32: the group's extremes are two
 // shuffles, and the eight key codes are one word.  A CTA takes a run of tokens;
 // its first threads find each token's sequence (a binary search in the starts),
-// page and row once for all heads.
+// page and row once for all heads.  Bound by the quantisation's instructions
+// when writing (67 % of issue slots) and by the rows' bytes when reading: 12,700
+// tokens of 8 heads of 128, bf16 in and fp32 out, take 26 and 28 us on a B200.
+// (Four columns a thread, each thread finding its row's place: 84 us for both.)
 //
 // Pages.  Reference counts, tables and lengths are small integers; one CTA
 // settles them (block scans over the counts, in page order, so that the lowest
-// free page is always the next one), and a second kernel moves the pages'
-// bytes with the whole GPU.
+// free page is always the next one; 7 us for 2600 pages, most of it the scans'
+// barriers), and a second kernel moves the pages' bytes with the whole GPU: 104 MB
+// of moved pages in 35 us, 5.9 TB/s read and written.
 #include <type_traits>
 
 #include "kv4.cuh"

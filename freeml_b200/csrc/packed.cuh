@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t clamped_rows(const uint32_t* starts, uint32_
 // (among equals, the sequences in order), so that no long one is left for the
 // end (sequence after sequence instead, each from its longest item on: 64 ragged
 // fp32 prompts 67 us, so 55; 12 grouped bf16 prompts of up to 4096 330 us, so
-// 290).  A bisection finds the weight from the sequences' lengths.  Called by a
+// 294).  A bisection finds the weight from the sequences' lengths.  Called by a
 // whole warp.
 __device__ inline PackedTile packed_tile(const PackedArgs& a, uint32_t idx)
 {

@@ -107,9 +107,9 @@ __device__ __forceinline__ void mma_tf32(uint32_t tmem_d, uint64_t da, uint64_t 
 }
 
 // The product (also with A read from TMEM: lane = row, one tf32 per 32-bit
-// column along K) and its commit from a whole warp, of which the hardware elects one lane (the
-// same one each time): operands are then the same in the warp for the compiler
-// too.  From a branch of one thread a product takes 80 to 130 cycles to issue,
+// column along K) and its commit from a whole warp, of which the hardware elects
+// one lane (the same one each time): operands are then the same in the warp for
+// the compiler too.  From a branch of one thread a product takes 80 to 130 cycles to issue,
 // more than a small one takes to run; so, 15 to 25.
 __device__ __forceinline__ void mma_tf32_elected(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                                  bool accumulate)
