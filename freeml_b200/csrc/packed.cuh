@@ -39,49 +39,65 @@ __device__ __forceinline__ uint32_t clamped_rows(const uint32_t* starts, uint32_
     return e > s ? e - s : 0u;
 }
 
-// Item number `idx`'s rows, by weight: item j of a sequence weighs j and the
-// keys before its first query, in items' tokens, and the heaviest come first
-// (among equals, the sequences in order), so that no long one is left for the
-// end (sequence after sequence instead, each from its longest item on: 64 ragged
-// fp32 prompts 67 us, so 55; 12 grouped bf16 prompts of up to 4096 330 us, so
-// 294).  A bisection finds the weight from the sequences' lengths.  Called by a
-// whole warp.
-__device__ inline PackedTile packed_tile(const PackedArgs& a, uint32_t idx)
+// Sequence b's rows; its work items weigh shift .. shift + n - 1: item j of a
+// sequence weighs j and the keys before its first query, in items' tokens.
+__device__ __forceinline__ void packed_sequence(const PackedArgs& a, uint32_t b, PackedTile* t, uint32_t* n,
+                                                uint32_t* shift)
 {
-    const uint32_t lane = threadIdx.x & 31u;
+    *n = *shift = 0;
+    if (b >= a.batch) return;
     auto steps = [&](uint32_t x) { return (uint32_t)((uint64_t)x * a.mul >> a.shift); };
-    // sequence b's items weigh shift .. shift + n - 1
-    auto sequence = [&](uint32_t b, PackedTile* t, uint32_t* n, uint32_t* shift) {
-        *n = *shift = 0;
-        if (b >= a.batch) return;
-        t->lq = clamped_rows(a.q_starts, b, a.q_rows, &t->q0);
-        *n = steps(t->lq + a.step - 1);
-        t->lk = t->lq;
-        t->k0 = t->q0;
-        if (a.k_starts == a.q_starts && a.k_rows == a.q_rows) return;
-        t->lk = clamped_rows(a.k_starts, b, a.k_rows, &t->k0);
-        if (t->lk > t->lq) *shift = steps(t->lk - t->lq);
-    };
-    PackedTile t{};
+    t->lq = clamped_rows(a.q_starts, b, a.q_rows, &t->q0);
+    *n = steps(t->lq + a.step - 1);
+    t->lk = t->lq;
+    t->k0 = t->q0;
+    if (a.k_starts == a.q_starts && a.k_rows == a.q_rows) return;
+    t->lk = clamped_rows(a.k_starts, b, a.k_rows, &t->k0);
+    if (t->lk > t->lq) *shift = steps(t->lk - t->lq);
+}
+
+// The number of items, and what they all weigh less than; by a whole warp.
+struct PackedTotals
+{
+    uint32_t items, top;
+};
+
+__device__ inline PackedTotals packed_totals(const PackedArgs& a)
+{
+    PackedTile t;
     uint32_t n, shift, top = 0, total = 0;
 #pragma unroll 4
-    for (uint32_t b = lane; b < a.batch; b += 32)
+    for (uint32_t b = threadIdx.x & 31u; b < a.batch; b += 32)
     {
-        sequence(b, &t, &n, &shift);
+        packed_sequence(a, b, &t, &n, &shift);
         total += n;
         if (n) top = max(top, n + shift);
     }
-    total = __reduce_add_sync(FULL_MASK, total);
-    uint32_t lo = 0, hi = __reduce_max_sync(FULL_MASK, top), before = 0;
+    return {__reduce_add_sync(FULL_MASK, total), __reduce_max_sync(FULL_MASK, top)};
+}
+
+// Item number `idx`'s rows: the heaviest items come first (among equals, the
+// sequences in order), so that no long one is left for the end (sequence after
+// sequence instead, each from its longest item on: 64 ragged fp32 prompts 67 us,
+// so 55; 12 grouped bf16 prompts of up to 4096 330 us, so 288; but 256 bf16 ones
+// of up to 64 tokens, where the order is nothing and the search is what a short
+// item waits for, 59, so 64).  A bisection finds the weight from the sequences'
+// lengths.  Called by a whole warp.
+__device__ inline PackedTile packed_tile(const PackedArgs& a, const PackedTotals& all, uint32_t idx)
+{
+    if (idx >= all.items) return PackedTile{};
+    const uint32_t lane = threadIdx.x & 31u;
+    PackedTile t{};
+    uint32_t n, shift, lo = 0, hi = all.top, before = 0;
     // more than `idx` items weigh lo or more, `before` <= idx weigh hi or more
-    while (idx < total && hi - lo > 1)
+    while (hi - lo > 1)
     {
         const uint32_t mid = lo + (hi - lo) / 2;
         uint32_t sum = 0;
 #pragma unroll 4
         for (uint32_t b = lane; b < a.batch; b += 32)
         {
-            sequence(b, &t, &n, &shift);
+            packed_sequence(a, b, &t, &n, &shift);
             if (n + shift > mid) sum += min(n, n + shift - mid);
         }
         sum = __reduce_add_sync(FULL_MASK, sum);
@@ -89,9 +105,9 @@ __device__ inline PackedTile packed_tile(const PackedArgs& a, uint32_t idx)
         else hi = mid, before = sum;
     }
     uint32_t left = idx - before;
-    for (uint32_t b0 = 0; idx < total && b0 < a.batch; b0 += 32)
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 32)
     {
-        sequence(b0 + lane, &t, &n, &shift);
+        packed_sequence(a, b0 + lane, &t, &n, &shift);
         const bool has = lo >= shift && lo - shift < n;
         const uint32_t with = __ballot_sync(FULL_MASK, has);
         if (left < (uint32_t)__popc(with))

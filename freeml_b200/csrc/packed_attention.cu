@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) packed_attention_kernel(T* __restrict__ o
     __shared__ PackedTile found;
     if (threadIdx.x < 32)
     {
-        const PackedTile t = packed_tile(a, blockIdx.x / (a.kv_heads * a.nchunk));
+        const PackedTile t = packed_tile(a, packed_totals(a), blockIdx.x / (a.kv_heads * a.nchunk));
         if (threadIdx.x == 0) found = t;
     }
     __syncthreads();

@@ -555,13 +555,14 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
     {
         // ---------------- the next item ----------------
         const uint32_t ny = a.kv_heads * a.nchunk;
+        const PackedTotals all = packed_totals(a);
         uint32_t asked = 0;
         bool more = true;
         uint32_t block = blockIdx.x;
         for (uint32_t k = 0; more;)
         {
             Item it;
-            it.p = packed_tile(a, block / ny);
+            it.p = packed_tile(a, all, block / ny);
             // ask for the next block while this one is worked out
             if (lane == 0)
             {

@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
         __shared__ PackedTile found;
         if (warp == 0)
         {
-            const PackedTile t = packed_tile(pk, blockIdx.x / (pk.kv_heads * pk.nchunk));
+            const PackedTile t = packed_tile(pk, packed_totals(pk), blockIdx.x / (pk.kv_heads * pk.nchunk));
             if (lane == 0) found = t;
         }
         __syncthreads();
