@@ -8,7 +8,8 @@
 // The sums over codes are products of 16-bit halves with fp32 accumulators
 // (mma.sync): the codes are the 16-row operand, 16 keys or 16 columns, and 8
 // query heads the 8 columns of the other.  The keys' pairs are an operand as
-// they lie: row (scale_0, minimum_0, scale_1, ...) times (0, sum_0 q, 0, ...).
+// they lie (16-bit types): row (scale_0, minimum_0, scale_1, ...) times (0, sum_0
+// q, 0, ...).
 //
 // Precision.  q is scaled by a power of two into the halves' range, and p is
 // taken against a reference exponent that keeps p and p times the scale there;
@@ -16,8 +17,9 @@
 //   fp32: q and p go in as two halves each, hi and the remainder lo (22 bits);
 //   codes are made normal halves about their middle (code - 8 for keys, - 7.5
 //   for values), or the sums over codes would be large numbers that the minima's
-//   sums take away again (64 sequences of up to 1600 keys: 2e-5 off; centred,
-//   9e-7, the formula in plain fp32 4e-7).
+//   sums take away again, and a group's middle, minimum + 8 scale, is formed in
+//   fp32 before it meets the query (64 sequences of up to 1600 keys: 2e-5 off;
+//   centred, 9e-7; with the middles, 3e-7, the formula in plain fp32 4e-7).
 //   16-bit types: q is a half exactly; a code needs one AND to be an operand,
 //   because bits 0..3 (4..7) of a half ARE the number code * 2^-24 (2^-20).
 //   Products of such small halves are exact to about 2^-20 only, well below
@@ -32,7 +34,7 @@
 // output in registers.  Segments of a split sequence leave partial results,
 // which a second kernel joins.  About 350 instructions per 16 keys keep 62 % (fp32)
 // and 55 % (16 bit) of the issue slots busy: 64 sequences of 1600 keys, 16 heads of
-// 64, fp32, take 65 us on a B200 (2.0 TB/s); 8 of up to 65537, 32 on 8 heads of 128,
+// 64, fp32, take 66 us on a B200 (2.0 TB/s); 8 of up to 65537, 32 on 8 heads of 128,
 // bf16, 81 us (3.4 TB/s).
 #include <type_traits>
 
@@ -336,6 +338,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     constexpr float LOW = FULL ? 1.f : 16.f;
     uint32_t qh[NG][2][2], ql[FULL ? NG : 1][2][2], ua[2];
     float qf, uf;
+    float2 qsum[FULL ? NG : 1];  // fp32: sum q of a group, heads 2 c and 2 c + 1, as the scores take it
     {
         float x[NG][8], top = 0.f, sum = 0.f;
 #pragma unroll
@@ -361,7 +364,9 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
             float s = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
             s += __shfl_xor_sync(FULL_MASK, s, 1);
             s += __shfl_xor_sync(FULL_MASK, s, 2);
-            if (c == (uint32_t)g) sum = s * down * 0.015625f;  // a quarter's pair is its group's
+            if constexpr (FULL)
+                qsum[g] = make_float2(s2 * __shfl_sync(FULL_MASK, s, 8 * c), s2 * __shfl_sync(FULL_MASK, s, 8 * c + 4));
+            else if (c == (uint32_t)g) sum = s * down * 0.015625f;  // a quarter's pair is its group's
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
@@ -371,8 +376,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 if constexpr (FULL) ql[g][h][0] = l0, ql[g][h][1] = l1;
             }
         }
-        // (scale, minimum) of group c times (8 sum, sum) where codes are centred, else (0, sum)
-        split2(make_float2(FULL ? 8.f * sum : 0.f, sum), &ua[0], &ua[1]);
+        split2(make_float2(0.f, sum), &ua[0], &ua[1]);  // times (scale, minimum) of group c
     }
     // the factors of heads 2 c, 2 c + 1, whose scores this thread has
     const float2 qf2 = make_float2(__shfl_sync(FULL_MASK, qf, 8 * c), __shfl_sync(FULL_MASK, qf, 8 * c + 4));
@@ -421,14 +425,18 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     load_words<NG>(t + KCODE + (16 * sub + 8 * k + n) * B::ROW + c * (4 * NG), w[k]);
                     load_words<NG>(t + KMETA + (16 * sub + 8 * k + n) * B::META, km[k]);
                 }
-                // the pair of group c; no such group: zeros (the query's side is 0 too, but 0 * NaN is not)
-                uint32_t pair[2] = {0u, 0u};
-                if (c < NG)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        pair[k] = *reinterpret_cast<const uint32_t*>(t + KMETA + (16 * sub + 8 * k + n) * B::META + 4 * c);
                 float du[4];
-                mma_f16_zero(du, pair[0], pair[1], pair[0], pair[1], ua[0], ua[1]);  // hi, then lo, along k
+                if constexpr (!FULL)
+                {
+                    // the pair of group c; no such group: zeros (the query's side is 0 too, but 0 * NaN is not)
+                    uint32_t pair[2] = {0u, 0u};
+                    if (c < NG)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            pair[k] =
+                                *reinterpret_cast<const uint32_t*>(t + KMETA + (16 * sub + 8 * k + n) * B::META + 4 * c);
+                    mma_f16_zero(du, pair[0], pair[1], pair[0], pair[1], ua[0], ua[1]);  // hi, then lo, along k
+                }
                 float2 tt[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
@@ -451,8 +459,27 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     tt[0] = fma2(make_float2(k0, k0), make_float2(d[0], d[1]), tt[0]);
                     tt[1] = fma2(make_float2(k1, k1), make_float2(d[2], d[3]), tt[1]);
                 }
-                s[0] = fma2(qf2, tt[0], make_float2(uf2.x * du[0], uf2.y * du[1]));
-                s[1] = fma2(qf2, tt[1], make_float2(uf2.x * du[2], uf2.y * du[3]));
+                if constexpr (FULL)
+                {
+                    // the groups' middles, minimum + 8 scale: the two would cancel in a product
+                    float2 mid[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                        {
+                            const float2 v = __half22float2(bits_half2(km[k][g]));  // scale, minimum
+                            const float m = fmaf(8.f, v.x, v.y);
+                            mid[k] = fma2(make_float2(m, m), qsum[g], mid[k]);
+                        }
+                    s[0] = fma2(qf2, tt[0], mid[0]);
+                    s[1] = fma2(qf2, tt[1], mid[1]);
+                }
+                else
+                {
+                    s[0] = fma2(qf2, tt[0], make_float2(uf2.x * du[0], uf2.y * du[1]));
+                    s[1] = fma2(qf2, tt[1], make_float2(uf2.x * du[2], uf2.y * du[3]));
+                }
             }
             // ---- the values' pairs of keys n, n + 8 ----
             uint32_t vm[2][NG];
