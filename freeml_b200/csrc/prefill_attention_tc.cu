@@ -618,25 +618,27 @@ __global__ void __launch_bounds__(PpShape<HD, PACKED>::THREADS, PpShape<HD, PACK
                         }
                 }
                 else
-#pragma unroll
-                for (int c = 0; c < KS; c += 32)
                 {
-                    uint32_t u[32];
-                    tmem_ld32_async(tx + c0 + c, u);
-                    if constexpr (SPLIT3)
-                    {
-                        uint32_t w[32];
-                        tmem_ld32_async(tx + Pp::PLO + c0 + c, w);
-                        tmem_wait_ld(u);
-                        tmem_wait_ld(w);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]) + __uint_as_float(w[i]);
-                    }
-                    else
+                    for (int c = 0; c < KS; c += 32)
                     {
-                        tmem_wait_ld(u);
+                        uint32_t u[32];
+                        tmem_ld32_async(tx + c0 + c, u);
+                        if constexpr (SPLIT3)
+                        {
+                            uint32_t w[32];
+                            tmem_ld32_async(tx + Pp::PLO + c0 + c, w);
+                            tmem_wait_ld(u);
+                            tmem_wait_ld(w);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]);
+                            for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]) + __uint_as_float(w[i]);
+                        }
+                        else
+                        {
+                            tmem_wait_ld(u);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(u[i]);
+                        }
                     }
                 }
                 const uint32_t k0 = t * PP_KT + c0;
