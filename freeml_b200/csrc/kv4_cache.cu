@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(PT) kv4_reserve_kernel(PageArgs a, const uint3
     }
     __syncthreads();
     bool ok = bad_s == 0;
+    __syncthreads();  // read by all before thread 0 may write it again
     if (ok && (carry > a.pages || !take_free(a.refs, a.pages, carry, fresh)))
     {
         ok = false;
@@ -457,7 +458,9 @@ __global__ void __launch_bounds__(PT) kv4_fork_kernel(PageArgs a, const uint32_t
         else rows[i] = min(a.lens[p], a.max_pages << a.page_shift);
     }
     __syncthreads();
-    if (bad_s == 0)
+    const bool slots_ok = bad_s == 0;
+    __syncthreads();  // read by all before a claim may write it: all take the same side of what follows
+    if (slots_ok)
     {
         // a child must be empty and named once: claim it
         uint32_t carry = 0;

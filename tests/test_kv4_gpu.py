@@ -437,6 +437,44 @@ def test_page_operations_that_cannot_be_carried_out_change_nothing():
     assert c.refs.tolist() == [2, 1, 1, 1] and c.table[1].tolist() == [0, 3, -1]
 
 
+def test_a_fork_of_thousands_is_refused_whole():
+    """One child among several thousand holds rows, or is named twice, or the
+    pages run out: the block that settles a fork takes its entries in turns,
+    and all of its threads must come to the same end."""
+    n = 2500
+    c = kv4.KV4Cache(1, 1, 32, n + 8, 16, 2 * n + 2, 2)
+    c.reserve(ints([20, 16]), ints([0, 1]))
+    before = [t.clone() for t in (c.refs, c.table, c.lens, c.pool)]
+
+    def refused(parents, children, bit):
+        c.fork(ints(parents), ints(children))
+        for t, u in zip((c.refs, c.table, c.lens, c.pool), before):
+            assert torch.equal(t, u)
+        assert int(c.status) == bit
+        c.status.zero_()
+
+    kids = list(range(2, n + 2))
+    for _ in range(20):
+        for at in (0, 31, 1023, 1024, n - 1):
+            refused([0] * n, kids[:at] + [1] + kids[at + 1:], kv4.BAD_SLOT)      # a child that holds rows
+            refused([0] * n, kids[:at] + [kids[at - 1]] + kids[at + 1:], kv4.BAD_SLOT)  # a child named twice
+            refused([0] * n, kids[:at] + [2 * n + 2] + kids[at + 1:], kv4.BAD_SLOT)  # no such slot
+        refused([0] * (n + 6), list(range(2, n + 8)), kv4.NO_PAGES)  # one page short
+    c.fork(ints([0] * n), ints(kids))
+    c.check()
+    assert c.refs[:3].tolist() == [n + 1, 1, 1] and int(c.refs.sum()) == n + 1 + 2 + n
+    assert c.table[2:n + 2, 1].tolist() == list(range(3, n + 3))
+    # the same of a reserve: more pages than are free, and than there are at all
+    before = [t.clone() for t in (c.refs, c.table, c.lens, c.pool)]
+    free = list(range(n + 2, 2 * n + 2))
+    for rows_each in (1, 32) * 20:
+        c.reserve(ints([rows_each] * n), ints(free))
+        for t, u in zip((c.refs, c.table, c.lens, c.pool), before):
+            assert torch.equal(t, u)
+        assert int(c.status) == kv4.NO_PAGES
+        c.status.zero_()
+
+
 def test_forked_sequences_go_their_own_ways():
     """A prompt forked in the middle of a page: both append, both attend to
     their own rows, and compaction after the parent's end changes nothing."""
