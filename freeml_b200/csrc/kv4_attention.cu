@@ -494,10 +494,11 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
 #pragma unroll
                         for (int g = 0; g < NG; ++g) vm[k][g] = 0u;
                     }
-            uint32_t big = 0;  // low 16 bits: the largest scale's, which order as the scales do
+            // the largest scale's bits, without the sign (a constant group's minimum may have been
+            // rounded up past it): they order as the scales' magnitudes do
+            uint32_t big = 0;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) big = __vimax3_u16x2(big, vm[0][g], vm[1][g]);
-            big &= 0xffffu;
+            for (int g = 0; g < NG; ++g) big = __vimax3_u32(big, vm[0][g] & 0x7fffu, vm[1][g] & 0x7fffu);
             const bool over = big >= limit;
             const float2 top2 = make_float2(fmaxf(s[0].x, s[1].x), fmaxf(s[0].y, s[1].y));
             if (__any_sync(FULL_MASK, over || top2.x > edge[0] || top2.y > edge[1]))

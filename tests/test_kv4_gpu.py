@@ -262,6 +262,35 @@ def test_attention_scores_and_values_of_many_sizes():
         check(run_attention(c, [n], q, 0.3), *attend64(q, ko, vo, [n], 0.3, "fp32"))
 
 
+def scale_bits(c, table, n, hd, page, values):
+    """The bits of the scales [n, kv, hd / 32] of one sequence's keys or values, as the pool holds them."""
+    raw = c.pool[0].cpu().numpy().reshape(c.pool.shape[1], c.pool.shape[2], 2, -1)[:, :, int(values), page * hd // 2:]
+    pairs = np.ascontiguousarray(raw).view(np.uint16).reshape(*raw.shape[:2], page, hd // 32, 2)
+    return np.stack([pairs[table[t // page], :, t % page, :, 0] for t in range(n)])
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kind", sorted(DT))
+def test_attention_over_constant_groups_with_negative_scales(kind, hd):
+    """A group's minimum is rounded to fp16, so that a constant group (0.3) may
+    lie below it: its scale is then negative, or -0 (3e-8)."""
+    n, page, kv = 200, 16, 2
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    k, v = torch.randn(n, kv, hd, generator=g, device="cuda"), torch.randn(n, kv, hd, generator=g, device="cuda")
+    for x in (k, v):
+        x[::3, :, :32] = 0.3
+        x[1::3, 0, hd - 32:] = 3e-8
+        x[150:, 1, :32] = -0.7002  # and to the end
+    c = kv4.KV4Cache(1, kv, hd, 20, page, 1, 20)
+    c.reserve(ints([n]))
+    c.append(0, k, v, starts_of([n]))
+    for values in (False, True):
+        bits = scale_bits(c, c.table[0].tolist(), n, hd, page, values)
+        assert (bits[0, :, 0] > 0x8000).all() and bits[1, 0, -1] == 0x8000 and (bits[150:, 1, 0] > 0x8000).all()
+    q = torch.randn(1, 3 * kv, hd, generator=g, device="cuda").to(DT[kind])
+    check(run_attention(c, [n], q, 0.2), *attend64(q, *held(c, [n], k), [n], 0.2, kind))
+
+
 def test_attention_passes_nan_on():
     hd = 32
     c = kv4.KV4Cache(1, 2, hd, 4, 16, 1, 4)
