@@ -12,8 +12,10 @@
 // q, 0, ...).
 //
 // Precision.  q is scaled by a power of two into the halves' range, and p is
-// taken against a reference exponent that keeps p and p times the scale there;
-// p enters the output and its sum alike, so that the reference cancels.
+// taken against a running maximum, 2^4 over which it moves; p enters the output and
+// its sum alike, so that the maximum cancels.  p times a scale is moved to
+// the top of the halves' range by a power of two of its own group of 32 columns (by
+// one for all, groups of a thousandth beside ones near fp16's limit were 1e-3 off).
 //   fp32: q and p go in as two halves each, hi and the remainder lo (22 bits);
 //   codes are made normal halves about their middle (code - 8 for keys, - 7.5
 //   for values), or the sums over codes would be large numbers that the minima's
@@ -167,15 +169,15 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// acc += a (hi + lo), the products' sum rounded into acc
+// acc += a (hi + lo) f, the products' sum rounded into acc; f a power of two
 __device__ __forceinline__ void add_products(float (&acc)[4], const uint32_t (&a)[4], const uint32_t (&hi)[2],
-                                             const uint32_t (&lo)[2])
+                                             const uint32_t (&lo)[2], float f)
 {
     float d[4];
     mma_f16_zero(d, a[0], a[1], a[2], a[3], lo[0], lo[1]);
     mma_f16(d, a, hi[0], hi[1]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) acc[x] += d[x];
+    for (int x = 0; x < 4; ++x) acc[x] = fmaf(d[x], f, acc[x]);
 }
 
 struct Segment
@@ -381,6 +383,8 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     // the factors of heads 2 c, 2 c + 1, whose scores this thread has
     const float2 qf2 = make_float2(__shfl_sync(FULL_MASK, qf, 8 * c), __shfl_sync(FULL_MASK, qf, 8 * c + 4));
     const float2 uf2 = make_float2(__shfl_sync(FULL_MASK, uf, 8 * c), __shfl_sync(FULL_MASK, uf, 8 * c + 4));
+    // heads past the group's last see no key
+    const float2 none2 = make_float2(2 * c < nq ? 0.f : -INFINITY, 2 * c + 1 < nq ? 0.f : -INFINITY);
 
     griddep_launch_dependents();
     // of heads 2 c, 2 c + 1: the reference exponent, and this thread's share of the sum
@@ -388,13 +392,15 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     float2 l = make_float2(0.f, 0.f);
     float acc[NG][2][4];  // columns 32 g + 4 n + 2 i (+ 1: the upper two) of both heads
     float2 u2[NG];        // sum p minimum (FULL: minimum + 7.5 scale) over this thread's keys
-    constexpr int CAP = 30;
-    int span = CAP + 100;  // a fresh maximum's p is 2^span, and no p passes 2^(span + 4); not chosen yet
-    uint32_t limit = 0;    // bits of a half that the values' scales stay below
+    // e of each group, in a float's place: p scale stays below 2^(e - 126) and goes in 2^(141 - e) times
+    // larger; at the least for p = 2^4 by the smallest scale
+    constexpr uint32_t LEAST = 107u << 23;
+    uint32_t unit[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
     {
         u2[g] = make_float2(0.f, 0.f);
+        unit[g] = LEAST;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 if constexpr (FULL)
                 {
                     // the groups' middles, minimum + 8 scale: the two would cancel in a product
-                    float2 mid[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    float2 mid[2] = {none2, none2};
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
 #pragma unroll
@@ -477,8 +483,8 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 }
                 else
                 {
-                    s[0] = fma2(qf2, tt[0], make_float2(uf2.x * du[0], uf2.y * du[1]));
-                    s[1] = fma2(qf2, tt[1], make_float2(uf2.x * du[2], uf2.y * du[3]));
+                    s[0] = fma2(qf2, tt[0], fma2(uf2, make_float2(du[0], du[1]), none2));
+                    s[1] = fma2(qf2, tt[1], fma2(uf2, make_float2(du[2], du[3]), none2));
                 }
             }
             // ---- the values' pairs of keys n, n + 8 ----
@@ -494,32 +500,24 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
 #pragma unroll
                         for (int g = 0; g < NG; ++g) vm[k][g] = 0u;
                     }
-            // the largest scale's bits, without the sign (a constant group's minimum may have been
-            // rounded up past it): they order as the scales' magnitudes do
-            uint32_t big = 0;
+            // the scales as their group's power of two leaves them (negative where a constant group's
+            // minimum was rounded up past it): with p of at most 2^4 below 2^15, or it is chosen again
+            float sc[2][NG], most = 0.f;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) big = __vimax3_u32(big, vm[0][g] & 0x7fffu, vm[1][g] & 0x7fffu);
-            const bool over = big >= limit;
-            const float2 top2 = make_float2(fmaxf(s[0].x, s[1].x), fmaxf(s[0].y, s[1].y));
-            if (__any_sync(FULL_MASK, over || top2.x > edge[0] || top2.y > edge[1]))
+            for (int g = 0; g < NG; ++g)
             {
-                float f = 1.f;  // of a smaller span
-                if (__any_sync(FULL_MASK, over))
-                {
-                    const uint32_t top = __reduce_max_sync(FULL_MASK, big);
-                    // scales below 2^(e + 1), with p at most 2^(span + 4): products below 2^15
-                    int e = (int)(__float_as_uint(low_half(top)) >> 23 & 255u) - 126;
-                    e = e < -24 ? -24 : e > 15 ? 15 : e;
-                    limit = e >= 15 ? 0x10000u : __half_as_ushort(__float2half_rz(__uint_as_float((uint32_t)(128 + e) << 23)));
-                    const int fresh = min(CAP, 10 - e);
-                    if (fresh < span)
-                    {
-                        f = __uint_as_float((uint32_t)(127 + max(fresh - span, -126)) << 23);
-                        ref[0] += (float)(span - fresh);
-                        ref[1] += (float)(span - fresh);
-                        span = fresh;
-                    }
-                }
+                const float up = __uint_as_float(0x86000000u - unit[g]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) sc[k][g] = low_half(vm[k][g]) * up;
+                most = fmaxf(most, fmaxf(fabsf(sc[0][g]), fabsf(sc[1][g])));
+            }
+            const float2 top2 = make_float2(fmaxf(s[0].x, s[1].x), fmaxf(s[0].y, s[1].y));
+            const bool over = most >= 2048.f, risen = top2.x > edge[0] || top2.y > edge[1];
+            bool moved = false, wide = false;
+            if (__any_sync(FULL_MASK, over || risen))
+            {
+                moved = __any_sync(FULL_MASK, risen);
+                wide = __any_sync(FULL_MASK, over);
                 float corr[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -528,13 +526,13 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                     mx = fmaxf(mx, __shfl_xor_sync(FULL_MASK, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(FULL_MASK, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(FULL_MASK, mx, 16));
-                    // the reference moves only when a p would pass 2^(span + 4)
-                    const bool need = mx > ref[h] + (float)(span + 4);
-                    const float fresh = need ? mx - (float)span : ref[h];
-                    corr[h] = need ? f * ex2(ref[h] - fresh) : f;
+                    // the reference moves only when a p would pass 2^4
+                    const bool need = mx > ref[h] + 4.f;
+                    const float fresh = need ? mx : ref[h];
+                    corr[h] = need ? ex2(ref[h] - fresh) : 1.f;
                     ref[h] = fresh;
                     base[h] = fresh == -INFINITY ? 0.f : fresh;  // no key yet: 2^(-inf - 0) = 0
-                    edge[h] = fresh + (float)(span + 4);
+                    edge[h] = fresh + 4.f;
                 }
                 l.x *= corr[0];
                 l.y *= corr[1];
@@ -554,6 +552,33 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
             for (int k = 0; k < 2; ++k) p[k] = make_float2(ex2(s[k].x - base[0]), ex2(s[k].y - base[1]));
             l.x += p[0].x + p[1].x;
             l.y += p[0].y + p[1].y;
+
+            if (moved || wide)
+            {
+                // their groups' exponents again: what the subtile's keys ask for, and, while the maximum
+                // stays, the earlier ones', with room for scales 2^6 larger.  A key that hardly counts asks
+                // for its product alone.
+                const float pm[2] = {fmaxf(p[0].x, p[0].y), fmaxf(p[1].x, p[1].y)};
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                {
+                    float big = __uint_as_float(LEAST);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        big = fmaxf(big, fabsf(low_half(vm[k][g])) * (pm[k] >= 0x1p-12f ? 16.f : pm[k]));
+                    const uint32_t field = (__reduce_max_sync(FULL_MASK, __float_as_uint(big)) & 0x7f800000u) + (6u << 23);
+                    const uint32_t to = moved ? field : max(unit[g], field);
+                    const float f = __uint_as_float(0x3f800000u + unit[g] - to), up = __uint_as_float(0x86000000u - to);
+                    unit[g] = to;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) sc[k][g] = low_half(vm[k][g]) * up;
+                    if constexpr (!FULL)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[g][j][x] *= f;
+                }
+            }
 
             // ---- output: codes of columns 32 g + 4 n + j of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9 ----
             uint32_t vw[4][(NG + 1) / 2];
@@ -593,7 +618,7 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 for (int k = 0; k < 2; ++k)
                 {
                     const float2 v = __half22float2(bits_half2(vm[k][g]));  // scale, minimum
-                    split2(mul2(p[k], make_float2(v.x, v.x)), &hi[k], &lo[k]);
+                    split2(mul2(p[k], make_float2(sc[k][g], sc[k][g])), &hi[k], &lo[k]);
                     hi[k] = transpose8(hi[k]);
                     lo[k] = transpose8(lo[k]);
                     const float mid = FULL ? fmaf(7.5f, v.x, v.y) : v.y;
@@ -603,8 +628,9 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 {
                     // the tensor cores' running sums are cut, not rounded: fp32
                     // sums of many keys are kept outside them
-                    add_products(acc[g][0], a0, hi, lo);
-                    add_products(acc[g][1], a1, hi, lo);
+                    const float down = __uint_as_float(unit[g] - 0x07000000u);  // 2^(e - 141)
+                    add_products(acc[g][0], a0, hi, lo, down);
+                    add_products(acc[g][1], a1, hi, lo, down);
                 }
                 else
                 {
@@ -625,13 +651,15 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
         l.x += __shfl_xor_sync(FULL_MASK, l.x, o);
         l.y += __shfl_xor_sync(FULL_MASK, l.y, o);
     }
-    const float lowf = FULL ? 1.f : 16777216.f, highf = FULL ? 1.f : 1048576.f;
     __syncthreads();  // the ring is free
     float* mine_o = reinterpret_cast<float*>(ring[warp]);
 #pragma unroll
     for (int g = 0; g < NG; ++g)
     {
         float2 u = u2[g];
+        // 16 bit: codes at 2^-24 and 2^-20, in the units of p scale
+        const float down = FULL ? 1.f : __uint_as_float(unit[g] - 0x07000000u);
+        const float lowf = FULL ? 1.f : 16777216.f * down, highf = FULL ? 1.f : 1048576.f * down;
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1)
         {

@@ -291,6 +291,30 @@ def test_attention_over_constant_groups_with_negative_scales(kind, hd):
     check(run_attention(c, [n], q, 0.2), *attend64(q, *held(c, [n], k), [n], 0.2, kind))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kind", sorted(DT))
+def test_attention_over_values_of_very_different_sizes(kind, hd):
+    """Groups of 32 columns that reach fp16's limit beside ones of a
+    thousandth, and single values at the limit among keys of a thousandth, which
+    the softmax all but leaves out: every column is as good as its own values."""
+    n, kv = 500, 2
+    g = torch.Generator(device="cuda").manual_seed(40 + hd)
+    k, v = (torch.randn(n, kv, hd, generator=g, device="cuda") for _ in range(2))
+    size = torch.tensor([1e-3, 1.5e4, 1.0, 1e-5], device="cuda").repeat_interleave(32)[:hd]
+    v *= size
+    q = torch.randn(1, 2 * kv, hd, generator=g, device="cuda").to(DT[kind])
+    for at in (0, 37, 250):  # keys that no query head of the group looks at
+        v[at] = torch.randn(kv, hd, generator=g, device="cuda") * 2e4
+        for h in range(kv):
+            k[at, h] = -12 * q[0, 2 * h:2 * h + 2].float().mean(0)
+    c = kv4.KV4Cache(1, kv, hd, 40, 16, 1, 40)
+    c.reserve(ints([n]))
+    c.append(0, k, v.clamp(-65504, 65504), starts_of([n]))
+    want, tol = attend64(q, *held(c, [n], k), [n], 0.3, kind)
+    # fp16 results below 2^-14 are rounded to multiples of 2^-24
+    check(run_attention(c, [n], q, 0.3), want, tol + (2.0 ** -25 if kind == "fp16" else 0))
+
+
 def test_attention_passes_nan_on():
     hd = 32
     c = kv4.KV4Cache(1, 2, hd, 4, 16, 1, 4)
