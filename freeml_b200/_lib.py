@@ -73,11 +73,13 @@ SIGNATURES = {
     "fml_attention_packed": (_I, [_P, _P, _P, _P, _I, _P, _P] + [_U32] * 10 + [_F, _I, _P]),
     "fml_kv4_block_bytes": (ctypes.c_size_t, [_U32, _U32]),
     "fml_kv4_append": (_I, [_P] * 6 + [_I, _P] + [_U32] * 10 + [_P]),
+    "fml_kv4_append_keeping": (_I, [_P] * 7 + [_I, _P] + [_U32] * 10 + [_P]),
     "fml_kv4_read": (_I, [_P, _P, _I] + [_P] * 5 + [_U32] * 10 + [_P]),
     "fml_attention_kv4_workspace_bytes": (ctypes.c_size_t, [_U32] * 6),
     "fml_attention_kv4": (_I, [_P, _P, _I, _U32, _U32] + [_P] * 4 + [_U32] * 8 + [_F, _P, ctypes.c_size_t, _P]),
     "fml_kv4_pages_workspace_bytes": (ctypes.c_size_t, [_U32, _U32]),
     "fml_kv4_reserve": (_I, [_P] * 5 + [_U32] * 5 + [_P, _P, ctypes.c_size_t, _P]),
+    "fml_kv4_reserve_keeping": (_I, [_P] * 6 + [_U32] * 5 + [_P, _P, ctypes.c_size_t, _P]),
     "fml_kv4_fork": (_I, [_P, _U32, _U64, _U64] + [_P] * 5 + [_U32] * 5 + [_P, _P, ctypes.c_size_t, _P]),
     "fml_kv4_free": (_I, [_P] * 4 + [_U32] * 4 + [_P, _P]),
     "fml_kv4_compact": (_I, [_P, _U32, _U64, _U64, _P, _P, _U32, _U32, _U32, _P, ctypes.c_size_t, _P]),

@@ -31,6 +31,7 @@ struct RowArgs
     T* k;
     T* v;
     const uint32_t* starts;
+    const uint32_t* kept;  // rows of a slot before kept[slot] are not written; null: all may be
     uint32_t batch, rows, ldk, ldv, tokens;  // tokens: rows of a CTA
     Kv4View c;
 };
@@ -39,8 +40,8 @@ constexpr uint32_t MAX_TOKENS = 16;
 
 // Where new row r lies: the offset of its page in the pool (head 0's block)
 // and its row within the page; false where it has no place.
-__device__ bool find_row(const Kv4View& c, const uint32_t* starts, uint32_t batch, uint32_t r, uint64_t block_bytes,
-                         uint64_t* at, uint32_t* row)
+__device__ bool find_row(const Kv4View& c, const uint32_t* starts, const uint32_t* kept, uint32_t batch, uint32_t r,
+                         uint64_t block_bytes, uint64_t* at, uint32_t* row)
 {
     uint32_t lo = 0, hi = batch;  // the last entry whose start is at most r
     while (hi - lo > 1)
@@ -54,6 +55,7 @@ __device__ bool find_row(const Kv4View& c, const uint32_t* starts, uint32_t batc
     const uint32_t slot = kv4_slot(c, lo), len = kv4_len(c, slot);
     if (end - r > len) return false;
     const uint32_t pos = len - (end - r);
+    if (kept && pos < kept[slot]) return false;
     const int32_t page = c.table[(uint64_t)slot * c.max_pages + (pos >> c.page_shift)];
     if (page < 0 || (uint32_t)page >= c.pages) return false;
     *at = (uint64_t)page * c.kv_heads * block_bytes;
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(RowArgs<T> a)
     {
         uint64_t at = 0;
         uint32_t row = 0;
-        const bool ok = find_row(a.c, a.starts, a.batch, r0 + threadIdx.x, block, &at, &row);
+        const bool ok = find_row(a.c, a.starts, a.kept, a.batch, r0 + threadIdx.x, block, &at, &row);
         at_s[threadIdx.x] = at;
         row_s[threadIdx.x] = ok ? row : ~0u;
     }
@@ -257,8 +259,8 @@ int check_view(const char* who, const void* pool, const void* table, const void*
 
 template <bool READ>
 int rows_entry(const char* who, void* pool, const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids,
-               void* k, void* v, int type, const uint32_t* starts, uint32_t batch, uint32_t rows, uint32_t ldk,
-               uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
+               const uint32_t* kept, void* k, void* v, int type, const uint32_t* starts, uint32_t batch, uint32_t rows,
+               uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
                uint32_t kv_heads, uint32_t head_dim, cudaStream_t st)
 {
     if (batch == 0 || rows == 0) return FML_OK;
@@ -275,8 +277,8 @@ int rows_entry(const char* who, void* pool, const int32_t* table, const uint32_t
     const Kv4View c{table, lens, slot_ids, pages, slots, max_pages, kv4_page_shift(page_size), kv_heads};
     auto go = [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        RowArgs<T> a{static_cast<unsigned char*>(pool), static_cast<T*>(k), static_cast<T*>(v), starts, batch, rows, ldk,
-                     ldv, tokens, c};
+        RowArgs<T> a{static_cast<unsigned char*>(pool), static_cast<T*>(k), static_cast<T*>(v), starts, kept, batch, rows,
+                     ldk, ldv, tokens, c};
         if (head_dim == 32) return launch_rows<T, 32, READ>(a, vec, st);
         if (head_dim == 64) return launch_rows<T, 64, READ>(a, vec, st);
         return launch_rows<T, 128, READ>(a, vec, st);
@@ -365,9 +367,10 @@ struct PageArgs
 constexpr uint32_t WS_HEAD = 16;
 
 // reserve: need[i] pages for entry i; the claims (top bit of lens) find slots
-// named twice.
+// named twice.  kept (or null) [slots]: the lengths where the call is refused; no
+// more than them where it is carried out.
 __global__ void __launch_bounds__(PT) kv4_reserve_kernel(PageArgs a, const uint32_t* slot_ids, const uint32_t* counts,
-                                                         uint32_t n, uint32_t* ws)
+                                                         uint32_t n, uint32_t* kept, uint32_t* ws)
 {
     __shared__ uint32_t bad_s;
     uint32_t* need = ws + WS_HEAD;  // exclusive sums, n + 1
@@ -425,6 +428,7 @@ __global__ void __launch_bounds__(PT) kv4_reserve_kernel(PageArgs a, const uint3
                 a.refs[fresh[j]] = 1;
             }
             a.lens[slot] = old + counts[i];
+            if (kept) kept[slot] = min(kept[slot], old);
         }
         return;
     }
@@ -432,7 +436,9 @@ __global__ void __launch_bounds__(PT) kv4_reserve_kernel(PageArgs a, const uint3
     for (uint32_t i = threadIdx.x; i < n; i += PT)
     {
         const uint32_t slot = slot_ids ? slot_ids[i] : i;
-        if (slot < a.slots) atomicAnd(&a.lens[slot], 0x7fffffffu);
+        if (slot >= a.slots) continue;
+        const uint32_t old = atomicAnd(&a.lens[slot], 0x7fffffffu) & 0x7fffffffu;
+        if (kept) kept[slot] = old;
     }
     if (threadIdx.x == 0) atomicOr(a.status, (int)bad_s);
 }
@@ -702,6 +708,22 @@ int check_pool(const char* who, const void* pool, uint32_t layers, uint64_t laye
     return FML_OK;
 }
 
+int reserve_entry(const char* who, int32_t* refs, int32_t* table, uint32_t* lens, uint32_t* kept,
+                  const uint32_t* slot_ids, const uint32_t* counts, uint32_t n, uint32_t pages, uint32_t slots,
+                  uint32_t max_pages, uint32_t page_size, int32_t* status, void* workspace, size_t workspace_bytes,
+                  cudaStream_t st)
+{
+    if (n == 0) return FML_OK;
+    FML_RC(check_pages(who, refs, table, pages, slots, max_pages, n, workspace, workspace_bytes));
+    FML_REQUIRE(lens && counts && status, "%s: null pointer", who);
+    FML_REQUIRE(kv4_page_shift(page_size) && (uint64_t)max_pages * page_size < (1ull << 31),
+                "%s: %u pages of %u rows a sequence", who, max_pages, page_size);
+    const PageArgs a{refs, table, lens, pages, slots, max_pages, kv4_page_shift(page_size), status};
+    kv4_reserve_kernel<<<1, PT, 0, st>>>(a, slot_ids, counts, n, kept, static_cast<uint32_t*>(workspace));
+    FML_LAUNCH_CHECK();
+    return FML_OK;
+}
+
 constexpr uint32_t COPY_CTAS = 148 * 8;
 
 }  // namespace
@@ -722,9 +744,22 @@ int fml_kv4_append(void* pool, const int32_t* table, const uint32_t* lens, const
                    uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
                    uint32_t kv_heads, uint32_t head_dim, fml_stream_t stream)
 {
-    return rows_entry<false>("fml_kv4_append", pool, table, lens, slot_ids, const_cast<void*>(k), const_cast<void*>(v),
-                             type, starts, batch, rows, ldk, ldv, pages, slots, max_pages, page_size, kv_heads,
-                             head_dim, as_stream(stream));
+    return rows_entry<false>("fml_kv4_append", pool, table, lens, slot_ids, nullptr, const_cast<void*>(k),
+                             const_cast<void*>(v), type, starts, batch, rows, ldk, ldv, pages, slots, max_pages,
+                             page_size, kv_heads, head_dim, as_stream(stream));
+}
+
+int fml_kv4_append_keeping(void* pool, const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids,
+                           const uint32_t* kept, const void* k, const void* v, int type, const uint32_t* starts,
+                           uint32_t batch, uint32_t rows, uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots,
+                           uint32_t max_pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim,
+                           fml_stream_t stream)
+{
+    if (batch == 0 || rows == 0) return FML_OK;
+    FML_REQUIRE(kept, "fml_kv4_append_keeping: null pointer");
+    return rows_entry<false>("fml_kv4_append_keeping", pool, table, lens, slot_ids, kept, const_cast<void*>(k),
+                             const_cast<void*>(v), type, starts, batch, rows, ldk, ldv, pages, slots, max_pages,
+                             page_size, kv_heads, head_dim, as_stream(stream));
 }
 
 int fml_kv4_read(void* k, void* v, int type, const void* pool, const int32_t* table, const uint32_t* lens,
@@ -732,8 +767,9 @@ int fml_kv4_read(void* k, void* v, int type, const void* pool, const int32_t* ta
                  uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
                  uint32_t kv_heads, uint32_t head_dim, fml_stream_t stream)
 {
-    return rows_entry<true>("fml_kv4_read", const_cast<void*>(pool), table, lens, slot_ids, k, v, type, starts, batch,
-                            rows, ldk, ldv, pages, slots, max_pages, page_size, kv_heads, head_dim, as_stream(stream));
+    return rows_entry<true>("fml_kv4_read", const_cast<void*>(pool), table, lens, slot_ids, nullptr, k, v, type, starts,
+                            batch, rows, ldk, ldv, pages, slots, max_pages, page_size, kv_heads, head_dim,
+                            as_stream(stream));
 }
 
 size_t fml_kv4_pages_workspace_bytes(uint32_t pages, uint32_t n)
@@ -747,15 +783,19 @@ int fml_kv4_reserve(int32_t* refs, int32_t* table, uint32_t* lens, const uint32_
                     uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
                     int32_t* status, void* workspace, size_t workspace_bytes, fml_stream_t stream)
 {
+    return reserve_entry("fml_kv4_reserve", refs, table, lens, nullptr, slot_ids, counts, n, pages, slots, max_pages,
+                         page_size, status, workspace, workspace_bytes, as_stream(stream));
+}
+
+int fml_kv4_reserve_keeping(int32_t* refs, int32_t* table, uint32_t* lens, uint32_t* kept, const uint32_t* slot_ids,
+                            const uint32_t* counts, uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages,
+                            uint32_t page_size, int32_t* status, void* workspace, size_t workspace_bytes,
+                            fml_stream_t stream)
+{
     if (n == 0) return FML_OK;
-    FML_RC(check_pages("fml_kv4_reserve", refs, table, pages, slots, max_pages, n, workspace, workspace_bytes));
-    FML_REQUIRE(lens && counts && status, "fml_kv4_reserve: null pointer");
-    FML_REQUIRE(kv4_page_shift(page_size) && (uint64_t)max_pages * page_size < (1ull << 31),
-                "fml_kv4_reserve: %u pages of %u rows a sequence", max_pages, page_size);
-    const PageArgs a{refs, table, lens, pages, slots, max_pages, kv4_page_shift(page_size), status};
-    kv4_reserve_kernel<<<1, PT, 0, as_stream(stream)>>>(a, slot_ids, counts, n, static_cast<uint32_t*>(workspace));
-    FML_LAUNCH_CHECK();
-    return FML_OK;
+    FML_REQUIRE(kept, "fml_kv4_reserve_keeping: null pointer");
+    return reserve_entry("fml_kv4_reserve_keeping", refs, table, lens, kept, slot_ids, counts, n, pages, slots,
+                         max_pages, page_size, status, workspace, workspace_bytes, as_stream(stream));
 }
 
 int fml_kv4_fork(void* pool, uint32_t layers, uint64_t layer_stride, uint64_t page_bytes, int32_t* refs,

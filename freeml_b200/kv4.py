@@ -7,7 +7,9 @@ slots: `table` int32 [slots, max_pages] (page numbers, -1 where there is none),
 `lens` int32 [slots].  `refs` int32 [pages] counts the slots that hold a page.
 Page operations take every layer's pool at once, [layers, pages, ...], and OR
 into `status` (int32 [1]) why a call could not be carried out; it then changes
-nothing.  `KV4Cache` keeps these tensors together.
+nothing.  `kept` int32 [slots], where it is passed to reserve and append, keeps
+an append behind a refused reserve off the rows that are there.  `KV4Cache`
+keeps these tensors together.
 """
 from __future__ import annotations
 
@@ -101,11 +103,23 @@ def _new_rows(what, pool, table, lens, k, v, starts, slot_ids):
     return pool.data_ptr(), table, lens, slot_ids, pk, pv, kind, _ints(starts, "starts"), tail
 
 
-def append(pool, table, lens, k, v, starts, slot_ids=None):
+def _kept(kept, slots):
+    if kept.shape[0] != slots:
+        _refuse(f"kept of {kept.shape[0]} slots, a table of {slots}")
+    return _ints(kept, "kept")
+
+
+def append(pool, table, lens, k, v, starts, slot_ids=None, kept=None):
     """Write each sequence's newest rows (fml_kv4_append): k, v [rows,
-    kv_heads, hd]; rows starts[b] .. starts[b + 1] - 1 are entry b's last."""
+    kv_heads, hd]; rows starts[b] .. starts[b + 1] - 1 are entry b's last.
+    Behind a refused reserve these places hold older rows: pass the reserve's
+    `kept`, or read its status in between."""
+    slots = table.shape[0]
     p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("append", pool, table, lens, k, v, starts, slot_ids)
-    call("fml_kv4_append", p, table, lens, slot_ids, pk, pv, kind, starts, *tail)
+    if kept is None:
+        call("fml_kv4_append", p, table, lens, slot_ids, pk, pv, kind, starts, *tail)
+    else:
+        call("fml_kv4_append_keeping", p, table, lens, slot_ids, _kept(kept, slots), pk, pv, kind, starts, *tail)
 
 
 def read(k, v, pool, table, lens, starts, slot_ids=None):
@@ -166,13 +180,18 @@ def _layers(pool, pages):
     _refuse(f"pool: expected a contiguous uint8 CUDA tensor [layers, {pages}, kv_heads, page_size, bytes]")
 
 
-def reserve(refs, table, lens, counts, page_size, status, slot_ids=None, workspace=None):
-    """lens[slot] += counts[i], with pages for the new rows (fml_kv4_reserve)."""
+def reserve(refs, table, lens, counts, page_size, status, slot_ids=None, workspace=None, kept=None):
+    """lens[slot] += counts[i], with pages for the new rows (fml_kv4_reserve);
+    kept: where an append with it may write (fml_kv4_reserve_keeping)."""
     n, pages = counts.shape[0], refs.shape[0]
     table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "reserve")
     hold, ws, size = _pages_workspace(refs, max(n, 1), workspace)
-    call("fml_kv4_reserve", _ints(refs, "refs"), table, lens, slot_ids, _ints(counts, "counts"), n, pages, slots, most,
-         page_size, _ints(status, "status"), ws, size, _stream(refs))
+    tail = (slot_ids, _ints(counts, "counts"), n, pages, slots, most, page_size, _ints(status, "status"), ws, size,
+            _stream(refs))
+    if kept is None:
+        call("fml_kv4_reserve", _ints(refs, "refs"), table, lens, *tail)
+    else:
+        call("fml_kv4_reserve_keeping", _ints(refs, "refs"), table, lens, _kept(kept, slots), *tail)
 
 
 def fork(pool, refs, table, lens, parents, children, status, workspace=None):
@@ -209,7 +228,8 @@ class KV4Cache:
     """The pools, tables, lengths and counts of one model's 4-bit cache.
 
     A step: reserve(counts); for each layer append(layer, k, v, starts) and
-    attention(layer, out, q).  check() reads the status word (it waits)."""
+    attention(layer, out, q).  check() reads the status word (it waits); until it
+    has told of a refused reserve, the rows that were there are not written."""
 
     def __init__(self, layers, kv_heads, head_dim, pages, page_size=64, slots=1, max_pages=None, device="cuda"):
         self.page_size = page_size
@@ -218,12 +238,13 @@ class KV4Cache:
         self.table = torch.full((slots, max_pages or pages), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(slots, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.kept = torch.zeros(slots, dtype=torch.int32, device=device)
 
     def reserve(self, counts, slot_ids=None):
-        reserve(self.refs, self.table, self.lens, counts, self.page_size, self.status, slot_ids)
+        reserve(self.refs, self.table, self.lens, counts, self.page_size, self.status, slot_ids, kept=self.kept)
 
     def append(self, layer, k, v, starts, slot_ids=None):
-        append(self.pool[layer], self.table, self.lens, k, v, starts, slot_ids)
+        append(self.pool[layer], self.table, self.lens, k, v, starts, slot_ids, self.kept)
 
     def read(self, layer, k, v, starts, slot_ids=None):
         read(k, v, self.pool[layer], self.table, self.lens, starts, slot_ids)
@@ -244,6 +265,7 @@ class KV4Cache:
         """Raise if an operation since the last check could not be carried out."""
         bits = int(self.status.item())
         self.status.zero_()
+        self.kept.zero_()
         why = [text for bit, text in ((NO_PAGES, "no free pages"), (BAD_SLOT, "a bad slot"),
                                       (ROW_FULL, "a sequence longer than its table row")) if bits & bit]
         if why:

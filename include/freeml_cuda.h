@@ -345,12 +345,21 @@ FML_API size_t fml_kv4_block_bytes(uint32_t head_dim, uint32_t page_size);
 /* Writes the newest rows of each sequence: entry b's rows starts[b] ..
  * starts[b + 1] - 1 of k and v ([rows][kv_heads][head_dim], row strides ldk /
  * ldv) become its rows lens - n .. lens - 1 (n their number; reserve first).
+ * The places come from lens alone: behind a reserve that was refused these are
+ * the rows that are there already, so read its status in between, or use the
+ * keeping form, which does not write a slot's rows before kept[slot] (device
+ * [slots], see the page operations).
  * fml_kv4_read writes the values that the same rows stand for into k and v. */
 FML_API int fml_kv4_append(void* pool, const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids,
                            const void* k, const void* v, int type, const uint32_t* starts, uint32_t batch,
                            uint32_t rows, uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots,
                            uint32_t max_pages, uint32_t page_size, uint32_t kv_heads, uint32_t head_dim,
                            fml_stream_t stream);
+FML_API int fml_kv4_append_keeping(void* pool, const int32_t* table, const uint32_t* lens, const uint32_t* slot_ids,
+                                   const uint32_t* kept, const void* k, const void* v, int type,
+                                   const uint32_t* starts, uint32_t batch, uint32_t rows, uint32_t ldk, uint32_t ldv,
+                                   uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,
+                                   uint32_t kv_heads, uint32_t head_dim, fml_stream_t stream);
 FML_API int fml_kv4_read(void* k, void* v, int type, const void* pool, const int32_t* table, const uint32_t* lens,
                          const uint32_t* slot_ids, const uint32_t* starts, uint32_t batch, uint32_t rows,
                          uint32_t ldk, uint32_t ldv, uint32_t pages, uint32_t slots, uint32_t max_pages,
@@ -376,7 +385,12 @@ FML_API int fml_attention_kv4(void* out, const void* q, int type, uint32_t ldo, 
  * it ORs why: FML_KV4_NO_PAGES, FML_KV4_BAD_SLOT (a slot out of range or
  * named twice, or a child that holds rows), FML_KV4_ROW_FULL (a sequence
  * longer than its table row).
- *   reserve  lens[slot] += counts[i], with pages for the new rows
+ *   reserve  lens[slot] += counts[i], with pages for the new rows.  The keeping
+ *            form also sets kept [slots] (device, zeros at first) for the slots
+ *            of the call: to their lens where it is refused, to their lens
+ *            before it, if that is less, where it is carried out.  The keeping
+ *            append behind it then writes nothing over what is there, without
+ *            a wait for the status; zero kept once the refusal is known
  *   fork     slot children[i] becomes a copy of slot parents[i]: full pages
  *            are shared (their counts rise), a page in use is copied, in
  *            every layer, so that both may append
@@ -395,6 +409,10 @@ FML_API int fml_kv4_reserve(int32_t* refs, int32_t* table, uint32_t* lens, const
                             const uint32_t* counts, uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages,
                             uint32_t page_size, int32_t* status, void* workspace, size_t workspace_bytes,
                             fml_stream_t stream);
+FML_API int fml_kv4_reserve_keeping(int32_t* refs, int32_t* table, uint32_t* lens, uint32_t* kept,
+                                    const uint32_t* slot_ids, const uint32_t* counts, uint32_t n, uint32_t pages,
+                                    uint32_t slots, uint32_t max_pages, uint32_t page_size, int32_t* status,
+                                    void* workspace, size_t workspace_bytes, fml_stream_t stream);
 FML_API int fml_kv4_fork(void* pool, uint32_t layers, uint64_t layer_stride, uint64_t page_bytes, int32_t* refs,
                          int32_t* table, uint32_t* lens, const uint32_t* parents, const uint32_t* children,
                          uint32_t n, uint32_t pages, uint32_t slots, uint32_t max_pages, uint32_t page_size,

@@ -108,3 +108,17 @@ def test_free_refuses():
         args[bad if bad != 9 else 8] = None
         assert rc("fml_kv4_free", *args) == 1
     assert rc("fml_kv4_free", None, None, None, None, 0, 0, 0, 0, None, None) == 0
+
+
+def test_the_keeping_forms_refuse():
+    """As the plain forms do, and without `kept`."""
+    rows = [P, P, P, None, P, P, P, 0, P, 2, 4, 128, 128, 4, 2, 2, 16, 2, 64, None]
+    for at in (0, 1, 2, 4, 5, 6, 8):
+        assert rc("fml_kv4_append_keeping", *rows[:at], None, *rows[at + 1:]) == 1
+    assert b"fml_kv4_append_keeping" in _lib.load().fml_last_error()
+    assert rc("fml_kv4_append_keeping", *rows[:4], None, *rows[5:9], 0, *rows[10:]) == 0
+    reserve = [P, P, P, P, P, P, 2, 16, 4, 4, 16, P, P, 1 << 20, None]
+    for at in (0, 1, 2, 3, 5, 11, 12):
+        assert rc("fml_kv4_reserve_keeping", *reserve[:at], None, *reserve[at + 1:]) == 1
+    assert b"fml_kv4_reserve_keeping" in _lib.load().fml_last_error()
+    assert rc("fml_kv4_reserve_keeping", *reserve[:6], 0, *reserve[7:]) == 0

@@ -528,6 +528,70 @@ def test_a_fork_of_thousands_is_refused_whole():
         c.status.zero_()
 
 
+def test_an_append_behind_a_refused_reserve_writes_nothing():
+    """A full pool, sequences that share their last full page: the rows of a
+    step that finds no page must not land on the newest rows there are."""
+    hd, kv, L, page = 64, 2, 2, 16
+    c = kv4.KV4Cache(L, kv, hd, 4, page, 4, 4)
+    k, v = rows([54], kv, hd, "fp32", 21)
+
+    def append(at, n, ids):
+        b = len(ids)
+        for l in range(L):
+            c.append(l, k[at:at + n].repeat(b, 1, 1), v[at:at + n].repeat(b, 1, 1), starts_of([n] * b), ints(ids))
+
+    c.reserve(ints([32]), ints([2]))
+    append(0, 32, [2])
+    c.fork(ints([2]), ints([0]))
+    c.reserve(ints([20]), ints([1]))
+    append(32, 20, [1])
+    c.check()
+    before = [t.clone() for t in (c.refs, c.table, c.lens, c.pool)]
+    q = torch.randn(3, 4, hd, device="cuda")
+    out = torch.empty_like(q)
+    c.attention(1, out, q, 0.2, ints([0, 1, 2]))
+    c.reserve(ints([1, 1, 1]), ints([0, 1, 2]))  # two pages more, none is free
+    append(52, 1, [0, 1, 2])
+    again = torch.empty_like(q)
+    c.attention(1, again, q, 0.2, ints([0, 1, 2]))
+    for t, u in zip((c.refs, c.table, c.lens, c.pool), before):
+        assert torch.equal(t, u)
+    assert torch.equal(out, again)
+    # a refusal for another reason, the row of a slot that is not in it is written
+    c.reserve(ints([1]), ints([1]))
+    c.reserve(ints([1, 99]), ints([0, 2]))
+    append(52, 1, [0, 1, 2])
+    assert c.lens.tolist() == [32, 21, 32, 0] and torch.equal(c.pool[:, :2], before[3][:, :2])
+    ko, vo = torch.empty(21, kv, hd, device="cuda"), torch.empty(21, kv, hd, device="cuda")
+    c.read(1, ko, vo, starts_of([21]), ints([1]))
+    np.testing.assert_array_equal(vo.cpu().numpy(), quantised(v[32:53].cpu().numpy()))
+    with pytest.raises(FmlError):
+        c.check()
+    # a slot that was refused goes on: freed and filled anew, and where its rows end
+    c.reserve(ints([1, 9]), ints([0, 7]))
+    c.free(ints([0, 1]))
+    c.reserve(ints([5, 3]), ints([0, 2]))
+    for l in range(L):
+        c.append(l, k[:8], v[:8], starts_of([5, 3]), ints([0, 2]))
+    for slot, n, want in ((0, 5, v[:5]), (2, 3, v[5:8]), (2, 35, torch.cat([v[:32], v[5:8]]))):
+        ko, vo = torch.empty(n, kv, hd, device="cuda"), torch.empty(n, kv, hd, device="cuda")
+        c.read(0, ko, vo, starts_of([n]), ints([slot]))
+        np.testing.assert_array_equal(vo.cpu().numpy(), quantised(want.cpu().numpy()))
+    # two reserves before their rows; rows written again after check() has told of a refusal
+    with pytest.raises(FmlError):
+        c.check()
+    c.reserve(ints([2]), ints([0]))
+    c.reserve(ints([3]), ints([0]))
+    c.append(0, k[10:15], v[10:15], starts_of([5]), ints([0]))
+    c.reserve(ints([99]), ints([0]))
+    with pytest.raises(FmlError):
+        c.check()
+    c.append(0, k[20:24], v[20:24], starts_of([4]), ints([0]))
+    ko, vo = torch.empty(10, kv, hd, device="cuda"), torch.empty(10, kv, hd, device="cuda")
+    c.read(0, ko, vo, starts_of([10]), ints([0]))
+    np.testing.assert_array_equal(vo.cpu().numpy(), quantised(torch.cat([v[:5], v[10:11], v[20:24]]).cpu().numpy()))
+
+
 def test_forked_sequences_go_their_own_ways():
     """A prompt forked in the middle of a page: both append, both attend to
     their own rows, and compaction after the parent's end changes nothing."""
