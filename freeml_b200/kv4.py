@@ -23,6 +23,12 @@ TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FML_TYPE_*
 NO_PAGES, BAD_SLOT, ROW_FULL = 1, 2, 4                           # FML_KV4_*
 
 
+def reasons(bits):
+    """A status word in words."""
+    return ", ".join(text for bit, text in ((NO_PAGES, "no free pages"), (BAD_SLOT, "a bad slot"),
+                                            (ROW_FULL, "a sequence longer than its table row")) if bits & bit)
+
+
 def _refuse(msg):
     raise FmlError(1, "kv4", msg)
 
@@ -266,7 +272,5 @@ class KV4Cache:
         bits = int(self.status.item())
         self.status.zero_()
         self.kept.zero_()
-        why = [text for bit, text in ((NO_PAGES, "no free pages"), (BAD_SLOT, "a bad slot"),
-                                      (ROW_FULL, "a sequence longer than its table row")) if bits & bit]
-        if why:
-            raise FmlError(5, "KV4Cache", ", ".join(why))
+        if bits:
+            raise FmlError(5, "KV4Cache", reasons(bits))

@@ -8,8 +8,10 @@ The forward is NanoLLM's (Examples/NanoLLM/NanoLLM.cpp:268-358) through the
 operators of matrix_ops, row by row the one that lm.NanoLM decodes; weights come
 in the same packed order.  A sequence lives in a slot of the cache and can be
 forked there (several continuations of one prompt share its full pages), freed,
-and the cache compacted.  lm.NanoLM, with an fp32 cache of equal prompts, is the
-faster loop; this one holds 5 bits a value where that holds 32.
+and the cache compacted.  A step or a fork that finds no free page raises and
+changes nothing; it can be made again once sequences have been freed.  lm.NanoLM,
+with an fp32 cache of equal prompts, is the faster loop; this one holds 5 bits a
+value where that holds 32.
 """
 from __future__ import annotations
 
@@ -43,30 +45,48 @@ class PagedLM:
         self.cache = kv4.KV4Cache(s.n_layer, s.n_head, self.hd, pages, page_size, slots, -(-s.context // page_size),
                                   device=params.device)
         self.length = [0] * slots  # the cache's lens, known to the host
+        self.outcome = torch.zeros(1, dtype=torch.int32, device=params.device)  # status word of this class's own calls
 
     def _ints(self, x):
         return torch.tensor(x, dtype=torch.int32, device=self.device)
+
+    def _refused(self):
+        """Why the page operation just made was refused, or 0 (waits for it)."""
+        bits = int(self.outcome.item())
+        if bits:
+            self.outcome.zero_()
+        return bits
 
     def _forward(self, tokens, positions, counts, slot_ids, prompt: bool):
         """Hidden rows of new tokens (entry b's counts[b] rows in order); their keys and values go into the cache."""
         s, d, T = self.shape, self.shape.d_model, len(tokens)
         new = lambda *dims: torch.empty(*dims, dtype=torch.float32, device=self.device)  # noqa: E731
         starts, ids = self._ints([0] + list(np.cumsum(counts))), self._ints(slot_ids)
-        self.cache.reserve(self._ints(counts), ids)
         x, where, h, y, qkv, f = new(T, d), new(T, d), new(T, d), new(T, d), new(T, 3 * d), new(T, 4 * d)
         M.GatherRows(x, self.tok, torch.tensor(tokens, dtype=torch.float32, device=self.device))
         M.GatherRows(where, self.pos, torch.tensor(positions, dtype=torch.float32, device=self.device))
         M.Add(x, x, where)
         q, k, v = (qkv.view(T, 3, s.n_head, self.hd)[:, i] for i in range(3))
         att, scale = y.view(T, s.n_head, self.hd), 1.0 / float(np.sqrt(self.hd))
+        c = self.cache
+        kv4.reserve(c.refs, c.table, c.lens, self._ints(counts), c.page_size, self.outcome, ids)
+        bits = self._refused()
+        if not bits:
+            for slot, n in zip(slot_ids, counts):
+                self.length[slot] += n
+        elif prompt:  # it reads no cache: check() tells that the slots have stayed empty
+            c.status.bitwise_or_(bits)
+        else:
+            raise kv4.FmlError(5, "PagedLM", "step: " + kv4.reasons(bits))
         for i, w in enumerate(self.layers):
             M.LayerNormOp(h, x, w["ln0"])
             M.Mul(qkv, h, w["qkv"])
-            self.cache.append(i, k, v, starts, ids)
+            if not bits:
+                kv4.append(c.pool[i], c.table, c.lens, k, v, starts, ids)
             if prompt:  # a prompt's rows see each other as they are
                 M.attention_packed(att, q, k, v, starts, scale)
             else:
-                self.cache.attention(i, att, q, scale, ids)
+                c.attention(i, att, q, scale, ids)
             M.Mul(h, y, w["proj"], M.RIGHT)
             M.Add(x, x, h)
             M.LayerNormOp(h, x, w["ln1"])
@@ -74,8 +94,6 @@ class PagedLM:
             M.GeluMat(f, f)
             M.Mul(h, f, w["mlp"])
             M.Add(x, x, h)
-        for slot, n in zip(slot_ids, counts):
-            self.length[slot] += n
         return x
 
     def _logits(self, rows):
@@ -86,7 +104,8 @@ class PagedLM:
         return out
 
     def prefill(self, prompts, slot_ids):
-        """Run prompts (lists of token ids, of any lengths) into empty slots; the logits after each one's last row."""
+        """Run prompts (lists of token ids, of any lengths) into empty slots; the logits after each one's last row.
+        Where the pages do not suffice all of the slots stay empty, which cache.check() tells (the logits are right)."""
         counts = [len(p) for p in prompts]
         if any(n < 1 or n > self.shape.context for n in counts) or any(self.length[i] for i in slot_ids) \
                 or len(slot_ids) != len(counts):
@@ -96,16 +115,20 @@ class PagedLM:
         return self._logits(x[(torch.tensor(np.cumsum(counts), device=self.device) - 1)].contiguous())
 
     def step(self, tokens, slot_ids):
-        """One more token of each slot; the logits after it."""
+        """One more token of each slot; the logits after it.  Raises, with nothing changed, where a page is missing."""
         positions = [self.length[i] for i in slot_ids]
         if any(p < 1 or p >= self.shape.context for p in positions):
             raise kv4.FmlError(1, "PagedLM", "step: a slot that is empty, or whose context is full")
         return self._logits(self._forward([int(t) for t in tokens], positions, [1] * len(slot_ids), slot_ids, prompt=False))
 
     def fork(self, parents, children):
-        self.cache.fork(self._ints(parents), self._ints(children))
-        for p, c in zip(parents, children):
-            self.length[c] = self.length[p]
+        c = self.cache
+        kv4.fork(c.pool, c.refs, c.table, c.lens, self._ints(parents), self._ints(children), self.outcome)
+        bits = self._refused()
+        if bits:
+            raise kv4.FmlError(5, "PagedLM", "fork: " + kv4.reasons(bits))
+        for parent, child in zip(parents, children):
+            self.length[child] = self.length[parent]
 
     def free(self, slot_ids):
         self.cache.free(self._ints(slot_ids))

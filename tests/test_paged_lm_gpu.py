@@ -96,6 +96,56 @@ def test_forks_continue_as_their_parent_does():
         torch.testing.assert_close(row.double(), step64(lm, 3, lm.length[slot] - 1, cached(lm, slot)), rtol=1e-3, atol=1e-3)
 
 
+def state_of(lm):
+    c = lm.cache
+    return [t.clone() for t in (c.refs, c.table, c.lens, c.pool)] + [list(lm.length)]
+
+
+def unchanged(lm, before):
+    now = state_of(lm)
+    return all(torch.equal(a, b) for a, b in zip(now[:4], before[:4])) and now[4] == before[4]
+
+
+def test_steps_and_forks_that_find_no_page():
+    """A step on a full cache raises and changes nothing, not even the full
+    last page that two forks share, and goes on once there is room."""
+    shape = SHAPES[0]
+    params = random_params(shape, 7)
+    lm = PagedLM(shape, params, pages=6, page_size=16, slots=5)
+    free = PagedLM(shape, params, pages=40, page_size=16, slots=5)
+    prompts = prompts_of(shape, [32, 47, 3], 2)
+    for one in (lm, free):
+        one.prefill(prompts, [0, 1, 4])
+        one.fork([0], [2])  # two full pages, shared
+    assert int((lm.cache.refs == 0).sum()) == 0
+    before = state_of(lm)
+    for _ in range(2):
+        with pytest.raises(FmlError):
+            lm.step([1, 2, 3], [0, 1, 2])
+        assert unchanged(lm, before)
+    with pytest.raises(FmlError):
+        lm.fork([1], [3])  # 47 rows: a page in use would be copied
+    assert unchanged(lm, before)
+    # prompts read no cache: their logits are right, their slot stays empty, and check() tells
+    logits = lm.prefill([prompts[2]], [3])
+    torch.testing.assert_close(logits, free.prefill([prompts[2]], [3]))
+    assert unchanged(lm, before)
+    with pytest.raises(FmlError):
+        lm.step([1], [3])
+    with pytest.raises(FmlError):
+        lm.cache.check()
+    lm.cache.check()
+    # a refusal that nobody has asked about yet is not a later step's
+    lm.cache.reserve(lm._ints([1]), lm._ints([9]))
+    torch.testing.assert_close(lm.step([5], [1]), free.step([5], [1]))
+    for one in (lm, free):
+        one.free([4, 1])
+    torch.testing.assert_close(lm.step([1, 2], [0, 2]), free.step([1, 2], [0, 2]))
+    assert lm.length == [33, 0, 33, 0, 0] and lm.cache.lens.tolist() == lm.length
+    with pytest.raises(FmlError):
+        lm.cache.check()
+
+
 def test_refusals_and_the_example():
     from freeml_b200 import paged_lm
     shape = SHAPES[0]
