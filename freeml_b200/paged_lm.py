@@ -50,6 +50,15 @@ class PagedLM:
     def _ints(self, x):
         return torch.tensor(x, dtype=torch.int32, device=self.device)
 
+    def _slots(self, what, slot_ids, each_once=True):
+        """The slots as whole numbers; refused unless they exist (and are named once): the cache would refuse them, or
+        take them for others than `length` does."""
+        ids = [int(i) for i in slot_ids]
+        if any(not 0 <= i < len(self.length) for i in ids) or (each_once and len(set(ids)) != len(ids)):
+            raise kv4.FmlError(1, "PagedLM", f"{what}: slots of 0 .. {len(self.length) - 1}"
+                                             f"{', each named once' if each_once else ''}")
+        return ids
+
     def _refused(self):
         """Why the page operation just made was refused, or 0 (waits for it)."""
         bits = int(self.outcome.item())
@@ -106,7 +115,7 @@ class PagedLM:
     def prefill(self, prompts, slot_ids):
         """Run prompts (lists of token ids, of any lengths) into empty slots; the logits after each one's last row.
         Where the pages do not suffice all of the slots stay empty, which cache.check() tells (the logits are right)."""
-        counts = [len(p) for p in prompts]
+        counts, slot_ids = [len(p) for p in prompts], self._slots("prefill", slot_ids)
         if any(n < 1 or n > self.shape.context for n in counts) or any(self.length[i] for i in slot_ids) \
                 or len(slot_ids) != len(counts):
             raise kv4.FmlError(1, "PagedLM", "prefill: prompts of 1 .. context tokens, one empty slot each")
@@ -116,12 +125,18 @@ class PagedLM:
 
     def step(self, tokens, slot_ids):
         """One more token of each slot; the logits after it.  Raises, with nothing changed, where a page is missing."""
+        slot_ids = self._slots("step", slot_ids)
         positions = [self.length[i] for i in slot_ids]
+        if len(tokens) != len(slot_ids):
+            raise kv4.FmlError(1, "PagedLM", f"step: {len(tokens)} tokens, {len(slot_ids)} slots")
         if any(p < 1 or p >= self.shape.context for p in positions):
             raise kv4.FmlError(1, "PagedLM", "step: a slot that is empty, or whose context is full")
         return self._logits(self._forward([int(t) for t in tokens], positions, [1] * len(slot_ids), slot_ids, prompt=False))
 
     def fork(self, parents, children):
+        parents, children = self._slots("fork", parents, False), self._slots("fork", children)
+        if len(parents) != len(children) or any(self.length[i] for i in children):
+            raise kv4.FmlError(1, "PagedLM", "fork: an empty child for each parent")
         c = self.cache
         kv4.fork(c.pool, c.refs, c.table, c.lens, self._ints(parents), self._ints(children), self.outcome)
         bits = self._refused()
@@ -131,6 +146,7 @@ class PagedLM:
             self.length[child] = self.length[parent]
 
     def free(self, slot_ids):
+        slot_ids = self._slots("free", slot_ids, False)
         self.cache.free(self._ints(slot_ids))
         for i in slot_ids:
             self.length[i] = 0

@@ -146,6 +146,27 @@ def test_steps_and_forks_that_find_no_page():
         lm.cache.check()
 
 
+def test_slots_that_are_not_as_they_should_be():
+    """Refused on the host: the device's lengths and the host's stay the same."""
+    shape = SHAPES[0]
+    lm = PagedLM(shape, random_params(shape, 8), pages=20, page_size=16, slots=4)
+    lm.prefill(prompts_of(shape, [20, 5], 3), [0, 1])
+    before = state_of(lm)
+    for bad in (lambda: lm.prefill([[1], [2]], [2, 2]), lambda: lm.prefill([[1]], [4]), lambda: lm.prefill([[1]], [-1]),
+                lambda: lm.prefill([[1]], [2, 3]), lambda: lm.step([1, 2], [0, 0]), lambda: lm.step([1], [-4]),
+                lambda: lm.step([1], [7]), lambda: lm.step([1, 2], [0]), lambda: lm.step([1], [0, 1]),
+                lambda: lm.fork([0], [1]), lambda: lm.fork([0, 0], [2, 2]), lambda: lm.fork([0], [-1]),
+                lambda: lm.fork([-4], [2]), lambda: lm.fork([0], [2, 3]), lambda: lm.fork([0, 1], [2]),
+                lambda: lm.free([4]), lambda: lm.free([0, -3])):
+        with pytest.raises(FmlError):
+            bad()
+        assert unchanged(lm, before)
+    lm.cache.check()
+    lm.free([0, 0])  # named twice, freed once
+    assert lm.length == [0, 5, 0, 0] and lm.cache.lens.tolist() == lm.length
+    lm.cache.check()
+
+
 def test_refusals_and_the_example():
     from freeml_b200 import paged_lm
     shape = SHAPES[0]
