@@ -36,9 +36,12 @@ def _refuse(msg):
 # The checks below run before every launch of a decode step: they are written
 # to cost little (the smallest calls take less time on the GPU than on the host).
 
-def _stream(t):
-    """The current stream of t's device, as the C ABI takes it."""
-    return _raw_stream(t.get_device())
+def _elsewhere(device, function, *args):
+    """function(*args) where its tensors' GPU is not the current one: with it current."""
+    if device < 0:
+        _refuse("expected CUDA tensors")
+    with torch.cuda.device(device):
+        function(*args)
 
 
 # torch.cuda.current_stream(device).cuda_stream builds a Stream object (3 us);
@@ -47,36 +50,36 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _rows(t, heads, hd, what):
-    """(pointer, row stride) of [rows, heads, hd] whose heads are dense."""
-    if t.is_cuda and t.dim() == 3:
+def _rows(t, heads, hd, what, device):
+    """(pointer, row stride) of [rows, heads, hd] on `device` whose heads are dense."""
+    if t.get_device() == device and t.dim() == 3:
         n, h, d = t.shape
         s0, s1, s2 = t.stride()
         if h == heads and d == hd and s2 == 1 and (s1 == hd or h == 1):
             return t.data_ptr(), s0 if n > 1 else max(s0, h * d)
-    _refuse(f"{what}: expected a CUDA tensor [rows, {heads}, {hd}] with dense heads")
+    _refuse(f"{what}: expected a tensor [rows, {heads}, {hd}] on GPU {device} with dense heads")
 
 
-def _ints(t, what, dims=1):
+def _ints(t, what, device, dims=1):
     if t is None:
         return None
-    if t.dtype is torch.int32 and t.is_cuda and t.dim() == dims and t.is_contiguous():
+    if t.dtype is torch.int32 and t.get_device() == device and t.dim() == dims and t.is_contiguous():
         return t.data_ptr()
-    _refuse(f"{what}: expected a contiguous int32 CUDA tensor of {dims} dimension(s)")
+    _refuse(f"{what}: expected a contiguous int32 tensor of {dims} dimension(s) on GPU {device}")
 
 
 def _geometry(pool, hd):
-    """(pages, kv_heads, page_size) of one layer's pool."""
-    if pool.dim() == 4 and pool.dtype is torch.uint8 and pool.is_cuda and pool.is_contiguous():
+    """(pages, kv_heads, page_size) of one layer's pool (on the current GPU: the caller has looked)."""
+    if pool.dim() == 4 and pool.dtype is torch.uint8 and pool.is_contiguous():
         pages, heads, page, width = pool.shape
         if width * 4 == hd * 5:
             return pages, heads, page
     _refuse(f"pool: expected a contiguous uint8 CUDA tensor [pages, kv_heads, page_size, {hd * 5 // 4}]")
 
 
-def _tables(table, lens, slot_ids, batch, what):
+def _tables(table, lens, slot_ids, batch, what, device):
     """(table, slots, max_pages, lens, slot_ids) as the C ABI takes them."""
-    at = _ints(table, "table", 2)
+    at = _ints(table, "table", device, 2)
     slots, most = table.shape
     if lens.shape[0] != slots:
         _refuse(f"{what}: lens of {lens.shape[0]} slots, a table of {slots}")
@@ -85,7 +88,7 @@ def _tables(table, lens, slot_ids, batch, what):
             _refuse(f"{what}: {batch} entries, {slots} slots")
     elif slot_ids.shape[0] != batch:
         _refuse(f"{what}: {batch} entries, {slot_ids.shape[0]} slot_ids")
-    return at, slots, most, _ints(lens, "lens"), _ints(slot_ids, "slot_ids")
+    return at, slots, most, _ints(lens, "lens", device), _ints(slot_ids, "slot_ids", device)
 
 
 def empty_pool(layers, pages, kv_heads, page_size, head_dim, device="cuda"):
@@ -95,24 +98,31 @@ def empty_pool(layers, pages, kv_heads, page_size, head_dim, device="cuda"):
     return torch.zeros(layers, pages, kv_heads, page_size, 5 * head_dim // 4, dtype=torch.uint8, device=device)
 
 
-def _new_rows(what, pool, table, lens, k, v, starts, slot_ids):
+def _workspace(t, device):
+    """(pointer, bytes) of a caller's workspace."""
+    if t.get_device() == device and t.is_contiguous():
+        return t.data_ptr(), t.numel() * t.element_size()
+    _refuse(f"workspace: expected a contiguous tensor on GPU {device}")
+
+
+def _new_rows(what, pool, table, lens, k, v, starts, slot_ids, device):
     """The arguments that append and read share."""
     hd = k.shape[-1]
     pages, heads, page = _geometry(pool, hd)
-    pk, ldk = _rows(k, heads, hd, "k")
-    pv, ldv = _rows(v, heads, hd, "v")
+    pk, ldk = _rows(k, heads, hd, "k", device)
+    pv, ldv = _rows(v, heads, hd, "v", device)
     kind, rows, batch = TYPES.get(k.dtype), k.shape[0], starts.shape[0] - 1
     if kind is None or v.dtype is not k.dtype or v.shape[0] != rows:
         _refuse(f"{what}: k and v differ, or their type")
-    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, what)
-    tail = (batch, rows, ldk, ldv, pages, slots, most, page, heads, hd, _stream(k))
-    return pool.data_ptr(), table, lens, slot_ids, pk, pv, kind, _ints(starts, "starts"), tail
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, what, device)
+    tail = (batch, rows, ldk, ldv, pages, slots, most, page, heads, hd, _raw_stream(device))
+    return pool.data_ptr(), table, lens, slot_ids, pk, pv, kind, _ints(starts, "starts", device), tail
 
 
-def _kept(kept, slots):
+def _kept(kept, slots, device):
     if kept.shape[0] != slots:
         _refuse(f"kept of {kept.shape[0]} slots, a table of {slots}")
-    return _ints(kept, "kept")
+    return _ints(kept, "kept", device)
 
 
 def append(pool, table, lens, k, v, starts, slot_ids=None, kept=None):
@@ -120,18 +130,25 @@ def append(pool, table, lens, k, v, starts, slot_ids=None, kept=None):
     kv_heads, hd]; rows starts[b] .. starts[b + 1] - 1 are entry b's last.
     Behind a refused reserve these places hold older rows: pass the reserve's
     `kept`, or read its status in between."""
-    slots = table.shape[0]
-    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("append", pool, table, lens, k, v, starts, slot_ids)
+    slots, device = table.shape[0], pool.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, append, pool, table, lens, k, v, starts, slot_ids, kept)
+    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("append", pool, table, lens, k, v, starts, slot_ids,
+                                                                     device)
     if kept is None:
         call("fml_kv4_append", p, table, lens, slot_ids, pk, pv, kind, starts, *tail)
     else:
-        call("fml_kv4_append_keeping", p, table, lens, slot_ids, _kept(kept, slots), pk, pv, kind, starts, *tail)
+        call("fml_kv4_append_keeping", p, table, lens, slot_ids, _kept(kept, slots, device), pk, pv, kind, starts, *tail)
 
 
 def read(k, v, pool, table, lens, starts, slot_ids=None):
     """The values that each sequence's newest rows stand for, into k and v
     (fml_kv4_read); rows as in append."""
-    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("read", pool, table, lens, k, v, starts, slot_ids)
+    device = pool.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, read, k, v, pool, table, lens, starts, slot_ids)
+    p, table, lens, slot_ids, pk, pv, kind, starts, tail = _new_rows("read", pool, table, lens, k, v, starts, slot_ids,
+                                                                     device)
     call("fml_kv4_read", pk, pv, kind, p, table, lens, slot_ids, starts, *tail)
 
 
@@ -143,14 +160,17 @@ def attention_workspace_bytes(batch, heads, kv_heads, head_dim, max_pages, page_
 def attention(out, q, pool, table, lens, scale, slot_ids=None, workspace=None):
     """One query row per sequence over the cache (fml_attention_kv4): q, out
     [batch, heads, hd]; entry b sees its lens keys."""
+    device = pool.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, attention, out, q, pool, table, lens, scale, slot_ids, workspace)
     batch, heads, hd = q.shape
     pages, kv_heads, page = _geometry(pool, hd)
-    pq, ldq = _rows(q, heads, hd, "q")
-    po, ldo = _rows(out, heads, hd, "out")
+    pq, ldq = _rows(q, heads, hd, "q", device)
+    po, ldo = _rows(out, heads, hd, "out", device)
     kind = TYPES.get(q.dtype)
     if kind is None or out.dtype is not q.dtype or out.shape[0] != batch:
         _refuse("attention: q and out differ, or their type")
-    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, "attention")
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, batch, "attention", device)
     size, ws = 0, None
     if workspace is None:
         size = attention_workspace_bytes(batch, heads, kv_heads, hd, most, page)
@@ -158,9 +178,9 @@ def attention(out, q, pool, table, lens, scale, slot_ids=None, workspace=None):
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
             ws = workspace.data_ptr()
     else:
-        ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        ws, size = _workspace(workspace, device)
     call("fml_attention_kv4", po, pq, kind, ldo, ldq, pool.data_ptr(), table, lens, slot_ids, batch, pages, slots, most,
-         page, heads, kv_heads, hd, float(scale), ws, size, _stream(q))
+         page, heads, kv_heads, hd, float(scale), ws, size, _raw_stream(device))
 
 
 @lru_cache(maxsize=256)
@@ -174,60 +194,69 @@ def _pages_workspace(refs, n, workspace):
         size = _pages_bytes(refs.shape[0], n)
         workspace = torch.empty(size, dtype=torch.uint8, device=refs.device)
         return workspace, workspace.data_ptr(), size
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace, *_workspace(workspace, refs.get_device())
 
 
-def _layers(pool, pages):
+def _layers(pool, pages, device):
     """(pointer, layers, bytes from one to the next, bytes of a page, rows of a page)"""
-    if pool.dim() == 5 and pool.dtype is torch.uint8 and pool.is_cuda and pool.is_contiguous():
+    if pool.dim() == 5 and pool.dtype is torch.uint8 and pool.get_device() == device and pool.is_contiguous():
         layers, n, heads, page, width = pool.shape
         if n == pages:
             return pool.data_ptr(), layers, n * heads * page * width, heads * page * width, page
-    _refuse(f"pool: expected a contiguous uint8 CUDA tensor [layers, {pages}, kv_heads, page_size, bytes]")
+    _refuse(f"pool: expected a contiguous uint8 tensor [layers, {pages}, kv_heads, page_size, bytes] on GPU {device}")
 
 
 def reserve(refs, table, lens, counts, page_size, status, slot_ids=None, workspace=None, kept=None):
     """lens[slot] += counts[i], with pages for the new rows (fml_kv4_reserve);
     kept: where an append with it may write (fml_kv4_reserve_keeping)."""
-    n, pages = counts.shape[0], refs.shape[0]
-    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "reserve")
+    n, pages, device = counts.shape[0], refs.shape[0], refs.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, reserve, refs, table, lens, counts, page_size, status, slot_ids, workspace, kept)
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "reserve", device)
     hold, ws, size = _pages_workspace(refs, max(n, 1), workspace)
-    tail = (slot_ids, _ints(counts, "counts"), n, pages, slots, most, page_size, _ints(status, "status"), ws, size,
-            _stream(refs))
+    refs, counts, status = _ints(refs, "refs", device), _ints(counts, "counts", device), _ints(status, "status", device)
+    tail = (slot_ids, counts, n, pages, slots, most, page_size, status, ws, size, _raw_stream(device))
     if kept is None:
-        call("fml_kv4_reserve", _ints(refs, "refs"), table, lens, *tail)
+        call("fml_kv4_reserve", refs, table, lens, *tail)
     else:
-        call("fml_kv4_reserve_keeping", _ints(refs, "refs"), table, lens, _kept(kept, slots), *tail)
+        call("fml_kv4_reserve_keeping", refs, table, lens, _kept(kept, slots, device), *tail)
 
 
 def fork(pool, refs, table, lens, parents, children, status, workspace=None):
     """Slot children[i] becomes a copy of slot parents[i] (fml_kv4_fork): full
     pages shared, a page in use copied in every layer of pool."""
-    n, pages = parents.shape[0], refs.shape[0]
-    base, layers, stride, page_bytes, page = _layers(pool, pages)
+    n, pages, device = parents.shape[0], refs.shape[0], refs.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, fork, pool, refs, table, lens, parents, children, status, workspace)
+    base, layers, stride, page_bytes, page = _layers(pool, pages, device)
     if children.shape[0] != n:
         _refuse(f"fork: {n} parents, {children.shape[0]} children")
-    table, slots, most, lens, _ = _tables(table, lens, None, 0, "fork")
+    table, slots, most, lens, _ = _tables(table, lens, None, 0, "fork", device)
     hold, ws, size = _pages_workspace(refs, max(n, 1), workspace)
-    call("fml_kv4_fork", base, layers, stride, page_bytes, _ints(refs, "refs"), table, lens, _ints(parents, "parents"),
-         _ints(children, "children"), n, pages, slots, most, page, _ints(status, "status"), ws, size, _stream(refs))
+    call("fml_kv4_fork", base, layers, stride, page_bytes, _ints(refs, "refs", device), table, lens,
+         _ints(parents, "parents", device), _ints(children, "children", device), n, pages, slots, most, page,
+         _ints(status, "status", device), ws, size, _raw_stream(device))
 
 
 def free(refs, table, lens, slot_ids, status):
     """Give the slots' pages back (fml_kv4_free)."""
-    n = slot_ids.shape[0]
-    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "free")
-    call("fml_kv4_free", _ints(refs, "refs"), table, lens, slot_ids, n, refs.shape[0], slots, most,
-         _ints(status, "status"), _stream(refs))
+    n, device = slot_ids.shape[0], refs.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, free, refs, table, lens, slot_ids, status)
+    table, slots, most, lens, slot_ids = _tables(table, lens, slot_ids, n, "free", device)
+    call("fml_kv4_free", _ints(refs, "refs", device), table, lens, slot_ids, n, refs.shape[0], slots, most,
+         _ints(status, "status", device), _raw_stream(device))
 
 
 def compact(pool, refs, table, workspace=None):
     """Move the used pages together, in every layer of pool (fml_kv4_compact)."""
-    pages = refs.shape[0]
-    base, layers, stride, page_bytes, _ = _layers(pool, pages)
+    pages, device = refs.shape[0], refs.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return _elsewhere(device, compact, pool, refs, table, workspace)
+    base, layers, stride, page_bytes, _ = _layers(pool, pages, device)
     hold, ws, size = _pages_workspace(refs, 0, workspace)
-    call("fml_kv4_compact", base, layers, stride, page_bytes, _ints(refs, "refs"), _ints(table, "table", 2), pages,
-         table.shape[0], table.shape[1], ws, size, _stream(refs))
+    call("fml_kv4_compact", base, layers, stride, page_bytes, _ints(refs, "refs", device),
+         _ints(table, "table", device, 2), pages, table.shape[0], table.shape[1], ws, size, _raw_stream(device))
 
 
 class KV4Cache:

@@ -145,11 +145,14 @@ def attention_packed(out, q, k, v, starts, scale, k_starts=None, mode=None):
     one QKV row will do); starts: int32 [batch + 1], the sequences' first rows;
     k_starts: the same for k and v where their rows lead the queries (a prompt
     run in chunks).  mode: FML_MATH_* of float32 (default: the library's)."""
+    device = q.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        return kv4._elsewhere(device, attention_packed, out, q, k, v, starts, scale, k_starts, mode)
     heads, kv_heads, hd = q.shape[1], k.shape[1], q.shape[2]
-    po, ldo = kv4._rows(out, heads, hd, "out")
-    pq, ldq = kv4._rows(q, heads, hd, "q")
-    pk, ldk = kv4._rows(k, kv_heads, hd, "k")
-    pv, ldv = kv4._rows(v, kv_heads, hd, "v")
+    po, ldo = kv4._rows(out, heads, hd, "out", device)
+    pq, ldq = kv4._rows(q, heads, hd, "q", device)
+    pk, ldk = kv4._rows(k, kv_heads, hd, "k", device)
+    pv, ldv = kv4._rows(v, kv_heads, hd, "v", device)
     kind, rows, k_rows, n = kv4.TYPES.get(q.dtype), q.shape[0], k.shape[0], starts.shape[0]
     if kind is None or out.dtype is not q.dtype or k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise FmlError(1, "matrix_ops", "attention_packed types")
@@ -158,8 +161,9 @@ def attention_packed(out, q, k, v, starts, scale, k_starts=None, mode=None):
         raise FmlError(1, "matrix_ops", "attention_packed shapes")
     if mode is None:
         mode = call("fml_get_math_mode")
-    call("fml_attention_packed", po, pq, pk, pv, kind, kv4._ints(starts, "starts"), kv4._ints(k_starts, "k_starts"),
-         n - 1, rows, k_rows, heads, kv_heads, hd, ldo, ldq, ldk, ldv, float(scale), mode, kv4._stream(q))
+    call("fml_attention_packed", po, pq, pk, pv, kind, kv4._ints(starts, "starts", device),
+         kv4._ints(k_starts, "k_starts", device), n - 1, rows, k_rows, heads, kv_heads, hd, ldo, ldq, ldk, ldv,
+         float(scale), mode, kv4._raw_stream(device))
 
 
 def attention_decode(out, q, kcache, vcache, lens, scale, workspace=None):
