@@ -55,9 +55,9 @@ def _rows(t, heads, hd, what, device):
     if t.get_device() == device and t.dim() == 3:
         n, h, d = t.shape
         s0, s1, s2 = t.stride()
-        if h == heads and d == hd and s2 == 1 and (s1 == hd or h == 1):
-            return t.data_ptr(), s0 if n > 1 else max(s0, h * d)
-    _refuse(f"{what}: expected a tensor [rows, {heads}, {hd}] on GPU {device} with dense heads")
+        if h == heads and d == hd and s2 == 1 and (s1 == hd or h == 1) and (n <= 1 or s0 < 1 << 32):
+            return t.data_ptr(), s0 if n > 1 else h * d
+    _refuse(f"{what}: expected a tensor [rows, {heads}, {hd}] on GPU {device} with dense heads, rows less than 2^32 apart")
 
 
 def _ints(t, what, device, dims=1):

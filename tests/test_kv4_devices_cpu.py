@@ -1,6 +1,6 @@
 """The 4-bit cache's and the packed attention's Python entry points: every
-tensor, a caller's workspace too, is on one GPU, and the call is made with that
-GPU current, on its stream.  Tensors are stand-ins, and the library's calls are
+tensor, a caller's workspace too, is on one GPU, the call is made with that GPU
+current, on its stream, and row strides fit the C ABI's 32 bits.  Tensors are stand-ins, and the library's calls are
 noted instead of made, so that no GPU is needed and none is reached."""
 import contextlib
 
@@ -77,7 +77,7 @@ def made(monkeypatch):
         yield
         current[0] = before
 
-    note = lambda name, *args: log.append((name, current[0], args[-1]))  # noqa: E731
+    note = lambda name, *args: log.append((name, current[0], args[-1], args))  # noqa: E731
     monkeypatch.setattr(kv4, "call", note)
     monkeypatch.setattr(matrix_ops, "call", note)
     monkeypatch.setattr(kv4, "_raw_stream", lambda d: 100 + d)
@@ -94,7 +94,7 @@ def test_the_tensors_gpu_is_made_current(name, made):
     for x in t.values():
         x.at, x.device = 1, torch.device("cuda", 1)
     run(t)
-    assert [m[1:] for m in made] == [(0, 100), (1, 101)]
+    assert [m[1:3] for m in made] == [(0, 100), (1, 101)]
 
 
 @pytest.mark.parametrize("name", sorted(CALLS))
@@ -116,3 +116,27 @@ def test_a_workspace_with_gaps_is_refused(name, made):
     with pytest.raises(FmlError):
         CALLS[name][1](t)
     assert not made
+
+
+@pytest.mark.parametrize("name,which,heads", [("append", "k", 2), ("append", "v", 2), ("read", "k", 2), ("attention", "q", 4),
+                                              ("attention", "out", 4), ("packed", "pq", 4), ("packed", "po", 4), ("packed", "k", 2)])
+def test_rows_too_far_apart_are_refused(name, which, heads, made):
+    """A stride of 2^32 elements and more would be cut to its low 32 bits."""
+    t = tensors()
+    for stride in (1 << 32, (1 << 32) + 64 * heads):
+        t[which] = Stand(t[which].shape, t[which].dtype, stride=[stride, 64, 1])
+        with pytest.raises(FmlError):
+            CALLS[name][1](t)
+    assert not made
+    t[which] = Stand(t[which].shape, t[which].dtype, stride=[(1 << 32) - 64, 64, 1])
+    CALLS[name][1](t)
+    assert (1 << 32) - 64 in made[0][3]
+
+
+def test_a_single_row_has_no_stride(made):
+    """One row of a tensor whose rows lie anywhere."""
+    t = tensors()
+    t["q"], t["out"] = (Stand((1, 4, 64), torch.float32, stride=[s, 64, 1]) for s in ((1 << 32) + 64, 256))
+    t["ids"] = i32(1)
+    CALLS["attention"][1](t)
+    assert made[0][3][3:5] == (256, 256)
