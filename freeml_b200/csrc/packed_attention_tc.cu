@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
                 mbar_arrive_expect_tx(&bars[B_CL], 16);
                 cuda::ptx::clusterlaunchcontrol_try_cancel(answer, &bars[B_CL]);
             }
+            ++asked;
             if (it.p.live)
             {
                 const uint32_t y = block % ny;
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
                 }
                 ++k;
             }
-            if (!wait(B_CL, asked++)) break;
+            if (!wait(B_CL, asked - 1)) break;
             const uint4 got = *answer;
             more = cuda::ptx::clusterlaunchcontrol_query_cancel_is_canceled(got);
             if (more) block = (uint32_t)cuda::ptx::clusterlaunchcontrol_query_cancel_get_first_ctaid_x<int>(got);
@@ -605,6 +606,8 @@ __global__ void __launch_bounds__(THREADS, 1) packed_attention_tc_kernel(const _
                 }
             }
         }
+        // an answer still on its way lands before the CTA exits (bounded; immediate on the normal path)
+        mbar_wait(&bars[B_CL], (asked - 1) & 1u);
     }
 
     tc_fence_before();
