@@ -24,8 +24,9 @@
 //   centred, 9e-7; with the middles, 3e-7, the formula in plain fp32 4e-7).
 //   16-bit types: q is a half exactly; a code needs one AND to be an operand,
 //   because bits 0..3 (4..7) of a half ARE the number code * 2^-24 (2^-20).
-//   Products of such small halves are exact to about 2^-20 only, well below
-//   the result's rounding.  p goes in as hi and lo all the same.
+//   Products of such small halves are exact to 2^-17 (2^-21) of 15 codes: enough
+//   for scores; the values' codes all go in at 2^-20 (a shift more).  p goes in as
+//   hi and lo all the same.
 //
 // Work.  What bounds it is the cache's bytes, and the instructions that unpack
 // them.  The keys of all sequences are cut into segments of about equal
@@ -157,11 +158,16 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w)
     return w & 0x00f000f0u;
 }
 
-// Codes 4..7 of a word's halves less 7.5, their middle.
-__device__ __forceinline__ uint32_t codes_middle(uint32_t w)
+// Two values' codes, bits 4..7 of a word's halves, as an operand: less 7.5, their
+// middle, or times 2^-20 (not, as keys' codes, some times 2^-24: 2^-17 of a group's
+// range is then lost, which values near zero, minimum and codes cancelling, show).
+template <bool FULL>
+__device__ __forceinline__ uint32_t value_codes(uint32_t w)
 {
-    return half2_bits(
-        __hfma2(bits_half2((w & 0x00f000f0u) | 0x64006400u), bits_half2(0x2c002c00u), bits_half2(0xd478d478u)));
+    if constexpr (FULL)
+        return half2_bits(
+            __hfma2(bits_half2((w & 0x00f000f0u) | 0x64006400u), bits_half2(0x2c002c00u), bits_half2(0xd478d478u)));
+    return w & 0x00f000f0u;
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src)
@@ -605,14 +611,10 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
                 // fp32: about 7.5, since what the codes' mean is off their middle stays in the sums over
                 // the keys until u2 takes it away again (two shifts more than about 8)
                 const uint32_t r0 = z0 >> 8, r1 = z1 >> 8;
-                const uint32_t a0[4] = {FULL ? codes_middle(z0 << 4) : codes_low<FULL>(z0),
-                                        FULL ? codes_middle(z0) : codes_high<FULL>(z0),
-                                        FULL ? codes_middle(z1 << 4) : codes_low<FULL>(z1),
-                                        FULL ? codes_middle(z1) : codes_high<FULL>(z1)};
-                const uint32_t a1[4] = {FULL ? codes_middle(z0 >> 4) : codes_low<FULL>(r0),
-                                        FULL ? codes_middle(r0) : codes_high<FULL>(r0),
-                                        FULL ? codes_middle(z1 >> 4) : codes_low<FULL>(r1),
-                                        FULL ? codes_middle(r1) : codes_high<FULL>(r1)};
+                const uint32_t a0[4] = {value_codes<FULL>(z0 << 4), value_codes<FULL>(z0), value_codes<FULL>(z1 << 4),
+                                        value_codes<FULL>(z1)};
+                const uint32_t a1[4] = {value_codes<FULL>(z0 >> 4), value_codes<FULL>(r0), value_codes<FULL>(z1 >> 4),
+                                        value_codes<FULL>(r1)};
                 uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -657,9 +659,8 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
     for (int g = 0; g < NG; ++g)
     {
         float2 u = u2[g];
-        // 16 bit: codes at 2^-24 and 2^-20, in the units of p scale
-        const float down = FULL ? 1.f : __uint_as_float(unit[g] - 0x07000000u);
-        const float lowf = FULL ? 1.f : 16777216.f * down, highf = FULL ? 1.f : 1048576.f * down;
+        // 16 bit: codes at 2^-20, in the units of p scale
+        const float f = FULL ? 1.f : 1048576.f * __uint_as_float(unit[g] - 0x07000000u);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1)
         {
@@ -670,8 +671,8 @@ __global__ void __launch_bounds__(32 * NW, ctas_per_sm(HD)) kv4_attention_kernel
         for (int h = 0; h < 2; ++h)
         {
             const float v = h ? u.y : u.x;
-            const float4 o = make_float4(fmaf(acc[g][0][h], lowf, v), fmaf(acc[g][0][h + 2], highf, v),
-                                         fmaf(acc[g][1][h], lowf, v), fmaf(acc[g][1][h + 2], highf, v));
+            const float4 o = make_float4(fmaf(acc[g][0][h], f, v), fmaf(acc[g][0][h + 2], f, v),
+                                         fmaf(acc[g][1][h], f, v), fmaf(acc[g][1][h + 2], f, v));
             *reinterpret_cast<float4*>(mine_o + (2 * c + h) * HD + 32 * g + 4 * n) = o;
         }
     }

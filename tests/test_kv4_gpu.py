@@ -216,6 +216,19 @@ def test_attention_of_long_sequences(hd, heads, kv):
         check(run_attention(c, lens, q, 0.11), *attend64(q, *held(c, lens, k), lens, 0.11, kind))
 
 
+@pytest.mark.parametrize("batch", [127, 128, 129, 300, 1000])
+@pytest.mark.parametrize("kind", sorted(DT))
+def test_attention_of_many_sequences(kind, batch):
+    """More entries than a block has threads to look their lengths up."""
+    lens = np.random.RandomState(batch).randint(0, 90, batch).tolist()
+    lens[batch // 2], lens[-1] = 2000, 700
+    c, k, v = cache_with(lens, 1, 32, 16, "fp32", 12)
+    q = torch.randn(batch, 3, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(13)).to(DT[kind])
+    out = run_attention(c, lens, q, 0.3)
+    check(out, *attend64(q, *held(c, lens, k), lens, 0.3, kind))
+    assert (out[[i for i, n in enumerate(lens) if n == 0]] == 0).all()
+
+
 def test_attention_through_slots_strides_and_missing_pages():
     """Entries in another order than their slots, a slot that does not exist,
     a strided query, a page that does not exist (its keys are masked)."""
