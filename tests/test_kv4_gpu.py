@@ -229,6 +229,35 @@ def test_attention_of_many_sequences(kind, batch):
     assert (out[[i for i, n in enumerate(lens) if n == 0]] == 0).all()
 
 
+def test_a_pool_past_four_gigabytes():
+    """Pages on both sides of 2^32 bytes: rows, attention, a fork's copy and compaction."""
+    hd, kv, page, pages = 128, 8, 128, 27000
+    c = kv4.KV4Cache(1, kv, hd, pages, page, 3, 4)
+    assert c.pool[0].numel() > 1 << 32
+    at = [26999, 5, 26500, 26214]  # 2^32 is in page 26214
+    c.table[0].copy_(ints(at))
+    c.refs[at] = 1
+    c.lens[0] = 400
+    k, v = rows([400], kv, hd, "fp32", 14)
+    c.append(0, k, v, starts_of([400]))
+    want_k, want_v = (torch.from_numpy(quantised(x.cpu().numpy())).cuda() for x in (k, v))
+    c.refs[:5] = 1  # the first free pages: 6, and, once the others have moved, a few more
+    c.fork(ints([0]), ints([2]))
+    c.check()
+    assert c.table[2].tolist() == [26999, 5, 26500, 6]
+    c.refs[:5] = 0
+    for _ in range(2):
+        q = torch.randn(2, 2 * kv, hd, device="cuda")
+        for slot in (0, 2):
+            ko, vo = torch.empty_like(k), torch.empty_like(v)
+            c.read(0, ko, vo, starts_of([400]), ints([slot]))
+            assert torch.equal(ko, want_k) and torch.equal(vo, want_v)
+        out = run_attention(c, [400, 400], q, 0.1, ints([0, 2]))
+        check(out, *attend64(q, want_k.repeat(2, 1, 1), want_v.repeat(2, 1, 1), [400, 400], 0.1, "fp32"))
+        c.compact()  # and once more as they lie then
+    assert sorted(set(c.table.flatten().tolist())) == [-1, 0, 1, 2, 3, 4]
+
+
 def test_attention_through_slots_strides_and_missing_pages():
     """Entries in another order than their slots, a slot that does not exist,
     a strided query, a page that does not exist (its keys are masked)."""

@@ -233,6 +233,17 @@ def test_many_sequences_and_a_stream_of_its_own():
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kind", sorted(DT))
+def test_scales_that_are_not_positive(kind, hd):
+    lq = [1, 200, 0, 77]
+    q, k, v = make(lq, lq, 6, 2, hd, kind, 17)
+    for scale, same in ((-0.15, -q), (0.0, 0 * q)):
+        out = torch.full_like(q, float("nan"))
+        matrix_ops.attention_packed(out, q, k, v, starts_of(lq), scale)
+        check(out, *reference(same, k, v, lq, lq, 0.15, kind))
+
+
 def test_no_wait_ran_out():
     import ctypes
     n = ctypes.c_uint64(1)
