@@ -229,6 +229,25 @@ def test_attention_of_many_sequences(kind, batch):
     assert (out[[i for i, n in enumerate(lens) if n == 0]] == 0).all()
 
 
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_attention_over_many_keys_of_about_equal_weight(kind, hd):
+    """Sums of 30,000 values whose mean is what is left: in the norm, no more
+    off than outputs rounded to their type (u / sqrt(3) at most) and a quarter
+    of an fp16 rounding for all else, however many keys a block sums up."""
+    n, kv, batch = 30000, 8, 24
+    c = kv4.KV4Cache(1, kv, hd, n // 64 + 1, 64, 1)
+    c.reserve(ints([n]))
+    k, v = rows([n], kv, hd, "fp32", 50 + hd)
+    c.append(0, k, v, starts_of([n]))
+    ko, vo = (x.double().transpose(0, 1) for x in held(c, [n], k))
+    q = (torch.randn(batch, kv, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(51)) * 0.5).to(DT[kind])
+    out = run_attention(c, [n], q, hd ** -0.5, ints([0] * batch))  # entries that read the same slot
+    want = (torch.softmax(q.double().transpose(0, 1) @ ko.transpose(1, 2) * hd ** -0.5, -1) @ vo).transpose(0, 1)
+    off = ((out.double() - want).norm() / want.norm()).item()
+    assert off <= U[kind] / math.sqrt(3) + 2.0 ** -13, off
+
+
 def test_a_pool_past_four_gigabytes():
     """Pages on both sides of 2^32 bytes: rows, attention, a fork's copy and compaction."""
     hd, kv, page, pages = 128, 8, 128, 27000
