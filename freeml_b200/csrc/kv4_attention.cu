@@ -13,15 +13,18 @@
 //
 // Precision.  q is scaled by a power of two into the halves' range, and p is
 // taken against a running maximum, 2^4 over which it moves; p enters the output and
-// its sum alike, so that the maximum cancels.  p times a scale is moved to
-// the top of the halves' range by a power of two of its own group of 32 columns (by
-// one for all, groups of a thousandth beside ones near fp16's limit were 1e-3 off).
+// its sum alike, so that the maximum cancels.  p times a scale is moved to the top
+// of the halves' range by a power of two of its own group of 32 columns (by one for
+// all, groups of a thousandth beside ones near fp16's limit were 1e-3 off).  Each 16
+// keys' products are a sum of their own, added in fp32.  What an output is off by
+// goes by the largest values of its group: one near 0 is minimum + code scale too.
 //   fp32: q and p go in as two halves each, hi and the remainder lo (22 bits);
 //   codes are made normal halves about their middle (code - 8 for keys, - 7.5
 //   for values), or the sums over codes would be large numbers that the minima's
 //   sums take away again, and a group's middle, minimum + 8 scale, is formed in
 //   fp32 before it meets the query (64 sequences of up to 1600 keys: 2e-5 off;
-//   centred, 9e-7; with the middles, 3e-7, the formula in plain fp32 4e-7).
+//   centred, 9e-7; with the middles, 3e-7; with a range for each group, 2.5e-7,
+//   the formula in plain fp32 4e-7).
 //   16-bit types: q is a half exactly; a code needs one AND to be an operand,
 //   because bits 0..3 (4..7) of a half ARE the number code * 2^-24 (2^-20).
 //   Products of such small halves are exact to 2^-17 (2^-21) of 15 codes: enough
@@ -33,12 +36,12 @@
 // length, one CTA each, so that ragged batches fill the GPU; a segment is
 // found from the lengths on the device.  Each of the CTA's warps streams its
 // own tiles (2560 bytes: 16, 32 or 64 keys) through a ring of cp.async stages,
-// masked keys filled with zeros, and keeps its own running maximum, sum and
-// output in registers.  Segments of a split sequence leave partial results,
-// which a second kernel joins.  About 350 instructions per 16 keys keep 62 % (fp32)
-// and 55 % (16 bit) of the issue slots busy: 64 sequences of 1600 keys, 16 heads of
-// 64, fp32, take 66 us on a B200 (2.0 TB/s); 8 of up to 65537, 32 on 8 heads of 128,
-// bf16, 81 us (3.4 TB/s).
+// whole ones, of which a count says the keys that are the sequence's, and keeps its
+// own running maximum, sum and output in registers.  Segments of a split sequence
+// leave partial results, which a second kernel joins.  About 380 (fp32, head dim 64)
+// and 455 (16 bit, 128) instructions per 16 keys keep 61 % and 59 % of the issue
+// slots busy: 64 sequences of 1600 keys, 16 heads of 64, fp32, take 69 us on a B200
+// (1.9 TB/s); 8 of up to 65537, 32 on 8 heads of 128, bf16, 92 us (3.0 TB/s).
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -53,7 +56,8 @@ constexpr int STAGES = 4;   // tiles in flight per warp
 constexpr int TILE = 2560;  // bytes of a tile
 constexpr uint32_t MIN_SEGMENT = 256;  // keys
 // CTAs an SM holds: head dim 128 needs the registers of 3 (8 long sequences of
-// grouped heads: 80 us against 92 at 4 with 128 registers a thread)
+// grouped heads, before sums were kept outside the products: 80 us against 92 at 4
+// with 128 registers a thread)
 constexpr int ctas_per_sm(int head_dim) { return head_dim == 128 ? 3 : 4; }
 
 template <typename T>

@@ -39,8 +39,12 @@
 // for: wait, ld, maximum, exponentials and st follow one another.  Tried and not
 // faster: four softmax warps a scheduler (a half's latency then bounds the two
 // buffers), turns at the exponentials, polynomials for a part of them.
-// Grouped bf16 prompts of up to 4096 (2.1e11 flops, head dim 128) take 253 us,
-// 0.83 PFLOP/s; fp16 ones of up to 1537, 16 heads of 64 (3.5e10), 123 us.
+// Grouped bf16 prompts of up to 4096 (2.1e11 flops, head dim 128) take 257 us,
+// 0.82 PFLOP/s; fp16 ones of up to 1537, 16 heads of 64 (3.5e10), 124 us.
+// P in 16 bits costs, in the norm, at most as much as the result's own rounding
+// (fp16 2.0e-4 -> 2.4e-4, bf16 1.6e-3 -> 2.0e-3 on these cases, about sqrt(2) times at the most).
+// As two halves it would fit the score buffer, but double the P V products and add
+// two conversions a score to the warps that the rest waits for.
 // Every wait is bounded and returns early once any role has recorded an expiry.
 // A wait tells neighbouring phases of a barrier apart only, so every role that
 // waits on a barrier follows all of its phases, or is never two behind.

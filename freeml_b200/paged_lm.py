@@ -10,8 +10,9 @@ in the same packed order.  A sequence lives in a slot of the cache and can be
 forked there (several continuations of one prompt share its full pages), freed,
 and the cache compacted.  A step or a fork that finds no free page raises and
 changes nothing; it can be made again once sequences have been freed.  lm.NanoLM,
-with an fp32 cache of equal prompts, is the faster loop; this one holds 5 bits a
-value where that holds 32.
+with an fp32 cache of equal prompts, is the faster loop (32 sequences, 512 wide, 8
+layers: 129,000 tokens/s on a B200, this one 23,000, for its launches from Python);
+this one holds 5 bits a value where that holds 32.
 """
 from __future__ import annotations
 

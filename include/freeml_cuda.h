@@ -367,7 +367,9 @@ FML_API int fml_kv4_read(void* k, void* v, int type, const void* pool, const int
 
 /* Attention of one query row per sequence over the cache: q, out [batch] rows
  * of [heads][head_dim], row strides ldq / ldo; entry b sees its lens keys (0
- * gives zeros).  The key range of long sequences is split across CTAs;
+ * gives zeros).  fp32 is kept to 22 bits of q and of the probabilities, sums to
+ * fp32, relative to the largest values of a column's group of 32.  The key range
+ * of long sequences is split across CTAs;
  * `workspace` (device, 16-byte aligned, any content, at least
  * fml_attention_kv4_workspace_bytes of these sizes, 0 where nothing can be
  * split) holds the splits' partial results until the call's kernels end. */
