@@ -45,6 +45,9 @@
 // (fp16 2.0e-4 -> 2.4e-4, bf16 1.6e-3 -> 2.0e-3 on these cases, about sqrt(2) times at the most).
 // As two halves it would fit the score buffer, but double the P V products and add
 // two conversions a score to the warps that the rest waits for.
+// O stays in TMEM over all keys, where the tensor cores cut their running sums: of
+// values whose mean is not 0, fp16 outputs are 2.7e-4 off behind 32,000 keys (plain
+// 2.2e-4) and 6.4e-4 behind 128,000; bf16 ones 1.87e-3, for a rounding of 1.79e-3.
 // Every wait is bounded and returns early once any role has recorded an expiry.
 // A wait tells neighbouring phases of a barrier apart only, so every role that
 // waits on a barrier follows all of its phases, or is never two behind.
